@@ -24,7 +24,7 @@
 #include <stdint.h>
 
 #define LFFW_FP8_ABI_MAJOR 1
-#define LFFW_FP8_ABI_MINOR 7
+#define LFFW_FP8_ABI_MINOR 8
 #define LFFW_FP8_API __attribute__((visibility("default")))
 #if defined(__cplusplus)
 #define LFFW_FP8_NOEXCEPT noexcept
@@ -402,6 +402,125 @@ LFFW_FP8_API int64_t lffw_skinny_packed_bytes(int64_t n, int64_t k, int32_t elem
 LFFW_FP8_API lffw_status lffw_pack_skinny_weights(const void *weight, int64_t n, int64_t k, int32_t elem_bytes,
                                                   void *packed, void *stream) LFFW_FP8_NOEXCEPT;
 
+/* ---- Scoring and training ---------------------------------------------------
+ * No counterpart in the reference: what a user needs to judge a (quantised) model's
+ * transcripts and to tune its norms and token table.  Rows are fp16 or bf16 (`dtype`,
+ * LFFW_DT_HALF or LFFW_DT_BF16); arithmetic is fp32.  Results do not depend on timing:
+ * no floating-point sum is formed in an order that varies between runs.  Every call
+ * waits for the work before it on `stream` before it reads anything, weights included.
+ * Calls on the same stream may share a workspace; calls that may overlap may not.
+ * Inputs, outputs and workspace may not overlap one another unless said otherwise.
+ *
+ * LayerNorm with its statistics kept (lffw_layer_norm's arithmetic, which stays the
+ * producer for the FP8 linears), per row of `cols`:
+ *   s = T(x + residual)  (s = x when residual is NULL; T rounds to `dtype`)
+ *   sum_out = s          (with residual; sum_out may be x or residual)
+ *   y = T((s - mean) * rstd * gamma + beta)
+ *   stats[row] = mean, stats[rows + row] = rstd = (var + epsilon)^-1/2
+ * Requirements: rows >= 1; 8 <= cols <= 4096, cols % 8 == 0; 16-byte aligned pointers;
+ * gamma, beta fp32 [cols]; stats fp32 [2, rows] (4-byte aligned); sum_out set exactly
+ * when residual is; epsilon finite and >= 0. */
+typedef struct lffw_layer_norm_train_args {
+    size_t struct_size; /* sizeof(lffw_layer_norm_train_args) */
+    int64_t rows, cols;
+    int32_t dtype;
+    const void *x;
+    const void *residual;
+    void *sum_out;
+    const float *gamma;
+    const float *beta;
+    float epsilon;
+    void *y;
+    float *stats;
+} lffw_layer_norm_train_args;
+
+LFFW_FP8_API lffw_status lffw_layer_norm_train(const lffw_layer_norm_train_args *args,
+                                               void *stream) LFFW_FP8_NOEXCEPT;
+
+/* Gradients of lffw_layer_norm_train.  s is its summed rows (x without a residual), with
+ * h = (s - mean) rstd and w = dy gamma:
+ *   dx     = T(rstd (w - mean(w) - h mean(w h)) + dsum)   (if dx)
+ *   dgamma = sum over rows of dy h, dbeta = sum over rows of dy, fp32   (both or neither)
+ * dsum (optional) is the gradient that arrives at sum_out by the residual stream; dx is
+ * then the gradient of x and of the residual alike, and may be dsum or dy itself.
+ * Requirements as above; dx and/or dgamma + dbeta set; with dgamma, workspace holds
+ * lffw_layer_norm_grad_workspace(rows, cols) bytes (0 for invalid arguments). */
+typedef struct lffw_layer_norm_grad_args {
+    size_t struct_size; /* sizeof(lffw_layer_norm_grad_args) */
+    int64_t rows, cols;
+    int32_t dtype;
+    const void *dy;
+    const void *s;
+    const float *gamma;
+    const float *stats;
+    const void *dsum;
+    void *dx;
+    float *dgamma;
+    float *dbeta;
+    void *workspace;
+    int64_t workspace_bytes;
+} lffw_layer_norm_grad_args;
+
+LFFW_FP8_API int64_t lffw_layer_norm_grad_workspace(int64_t rows, int64_t cols) LFFW_FP8_NOEXCEPT;
+LFFW_FP8_API lffw_status lffw_layer_norm_grad(const lffw_layer_norm_grad_args *args,
+                                              void *stream) LFFW_FP8_NOEXCEPT;
+
+/* Losses over the vocabulary from final states x [rows, width] and a token table
+ * weight [vocab, width] (the tied logits weight), z = x weight^T, without the logits:
+ *   labels (teacher_entries == 0): int32 or int64 (`label_bytes` 4 or 8) per row;
+ *     lse = log sum_v exp(z_v), losses = lse - z_label
+ *     A row whose label is ignore_index has loss 0 and takes no part in the gradients.
+ *   teacher (1 <= teacher_entries <= 256): tokens int32 and logits (`teacher_dtype`
+ *     LFFW_DT_FLOAT, HALF or BF16) [rows, teacher_entries], with temperature T:
+ *     t = softmax over the row's entries of logits / T,  lse = log sum_v exp(z_v / T)
+ *     losses = T^2 sum_j t_j (log t_j - z_j / T + lse)   (T^2 KL(teacher || student))
+ *     Entries with a negative token or a logit of -infinity are left out; a row with
+ *     none has loss 0 and takes no part in the gradients.  A token may occur twice.
+ * A label or token outside the vocabulary is treated as ignored (left out) and sets the
+ * error that lffw_vocab_loss_error reads.  Whatever the states of rows without a target
+ * hold, NaN included, reaches no gradient.
+ * lffw_vocab_loss writes losses and lse (fp32 [rows], both required).
+ * lffw_vocab_loss_grad reads lse and dloss (fp32 [rows], the gradients of the losses)
+ * and writes, in `dtype`, dx [rows, width] and/or dweight [vocab, width]:
+ *   G = dloss T (exp(z / T - lse) - t),  dx = G weight,  dweight = G^T x
+ * G is formed piece by piece over the vocabulary and held in 16 bits (scaled by a power of
+ * two so that fp16 neither overflows nor loses small probabilities); sums are fp32.
+ * workspace holds lffw_vocab_loss_workspace(args, 0 for the loss, 1 for the gradients)
+ * bytes (0 for invalid arguments; it depends on the shape, the targets and, for the
+ * gradients, on whether dx is set, not on the contents).
+ * Requirements: 1 <= rows <= 2^22; 1 <= vocab <= 2^22; 8 <= width <= 2^16, width % 8 == 0;
+ * 16-byte aligned x, weight, dx, dweight; a workspace on a 256-byte boundary;
+ * temperature in [2^-10, 2^10], exactly 1 with labels. */
+typedef struct lffw_vocab_loss_args {
+    size_t struct_size; /* sizeof(lffw_vocab_loss_args) */
+    int64_t rows, width, vocab;
+    int32_t dtype;
+    const void *x;
+    const void *weight;
+    const void *labels;
+    int32_t label_bytes;
+    int64_t ignore_index;
+    int32_t teacher_entries;
+    int32_t teacher_dtype;
+    const int32_t *teacher_tokens;
+    const void *teacher_logits;
+    float temperature;
+    float *losses;
+    float *lse;
+    const float *dloss;
+    void *dx;
+    void *dweight;
+    void *workspace;
+    int64_t workspace_bytes;
+} lffw_vocab_loss_args;
+
+LFFW_FP8_API int64_t lffw_vocab_loss_workspace(const lffw_vocab_loss_args *args, int32_t grad) LFFW_FP8_NOEXCEPT;
+LFFW_FP8_API lffw_status lffw_vocab_loss(const lffw_vocab_loss_args *args, void *stream) LFFW_FP8_NOEXCEPT;
+LFFW_FP8_API lffw_status lffw_vocab_loss_grad(const lffw_vocab_loss_args *args, void *stream) LFFW_FP8_NOEXCEPT;
+/* Reads and clears the current device's token error: 0 none, 1 a label or teacher token
+ * outside the vocabulary.  Synchronises with the device. */
+LFFW_FP8_API lffw_status lffw_vocab_loss_error(int32_t *code) LFFW_FP8_NOEXCEPT;
+
 /* GELU with every graph edge rounded to fp16, elementwise on `count` halves:
  * y = (x*0.5)*(1 + erf(x*fp16(2^-1/2))) (graph::gelu, network_graph.cpp:168-180).
  * The same device code as the fused GEMM epilogue. */
@@ -462,7 +581,7 @@ LFFW_FP8_API lffw_status lffw_fp8_linear_half_static(const uint16_t *x, int64_t 
  * adapter forwards createPlugin / onShapeChange / getWorkspaceSize / enqueue to
  * these calls one to one.  Enum values equal TensorRT's (DataType,
  * TensorFormat, PluginFieldType, TensorRTPhase). */
-enum { LFFW_DT_FLOAT = 0, LFFW_DT_HALF = 1, LFFW_DT_INT8 = 2, LFFW_DT_INT32 = 3, LFFW_DT_FP8 = 6 };
+enum { LFFW_DT_FLOAT = 0, LFFW_DT_HALF = 1, LFFW_DT_INT8 = 2, LFFW_DT_INT32 = 3, LFFW_DT_FP8 = 6, LFFW_DT_BF16 = 7 };
 enum { LFFW_FORMAT_LINEAR = 0, LFFW_FORMAT_CHW2 = 1 };
 enum {
     LFFW_FIELD_FLOAT16 = 0, LFFW_FIELD_FLOAT32 = 1, LFFW_FIELD_FLOAT64 = 2, LFFW_FIELD_INT8 = 3,

@@ -8,6 +8,7 @@ Modules:
   fp8      Q/DQ linear host API mirroring the reference's _Fp8Graph, plus the
            LayerNorm, attention and fp16 plugin calls; the TensorRT plugin
            creators are restated in the C ABI itself (lffw_plugin_*)
+  training LayerNorm, token cross entropy and distillation with their gradients
   scales   the reference's FP8 activation-scale file loader
   replicas one process per GPU: rank environment, batch shards, max-over-ranks
   build    in-tree nvcc build of liblffw_b200.so

@@ -29,7 +29,7 @@ EPILOGUE_GELU = 1
 WEIGHTS_ROW_MAJOR = 0
 WEIGHTS_SKINNY_TILES = 1
 
-DT_FLOAT, DT_HALF, DT_INT8, DT_INT32, DT_FP8 = 0, 1, 2, 3, 6
+DT_FLOAT, DT_HALF, DT_INT8, DT_INT32, DT_FP8, DT_BF16 = 0, 1, 2, 3, 6, 7
 FORMAT_LINEAR, FORMAT_CHW2 = 0, 1
 FIELD_FLOAT16, FIELD_FLOAT32, FIELD_FLOAT64, FIELD_INT8, FIELD_INT16, FIELD_INT32, FIELD_CHAR = range(7)
 PHASE_BUILD, PHASE_RUNTIME = 0, 1
@@ -175,6 +175,69 @@ class DecoderSelfAttentionArgs(ctypes.Structure):
     ]
 
 
+class LayerNormTrainArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_size_t),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("sum_out", ctypes.c_void_p),
+        ("gamma", ctypes.c_void_p),
+        ("beta", ctypes.c_void_p),
+        ("epsilon", ctypes.c_float),
+        ("y", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+    ]
+
+
+class LayerNormGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_size_t),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("dy", ctypes.c_void_p),
+        ("s", ctypes.c_void_p),
+        ("gamma", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("dsum", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+        ("dgamma", ctypes.c_void_p),
+        ("dbeta", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+class VocabLossArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_size_t),
+        ("rows", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("labels", ctypes.c_void_p),
+        ("label_bytes", ctypes.c_int32),
+        ("ignore_index", ctypes.c_int64),
+        ("teacher_entries", ctypes.c_int32),
+        ("teacher_dtype", ctypes.c_int32),
+        ("teacher_tokens", ctypes.c_void_p),
+        ("teacher_logits", ctypes.c_void_p),
+        ("temperature", ctypes.c_float),
+        ("losses", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("dloss", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+        ("dweight", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
 class PluginField(ctypes.Structure):
     _fields_ = [
         ("name", ctypes.c_char_p),
@@ -238,6 +301,13 @@ def library() -> ctypes.CDLL:
         "lffw_decoder_self_attention": ([ctypes.POINTER(DecoderSelfAttentionArgs), _vp], _i32),
         "lffw_greedy_select": ([_vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp], _i32),
         "lffw_decoder_error": ([ctypes.POINTER(_i32)], _i32),
+        "lffw_layer_norm_train": ([ctypes.POINTER(LayerNormTrainArgs), _vp], _i32),
+        "lffw_layer_norm_grad_workspace": ([_i64, _i64], _i64),
+        "lffw_layer_norm_grad": ([ctypes.POINTER(LayerNormGradArgs), _vp], _i32),
+        "lffw_vocab_loss_workspace": ([ctypes.POINTER(VocabLossArgs), _i32], _i64),
+        "lffw_vocab_loss": ([ctypes.POINTER(VocabLossArgs), _vp], _i32),
+        "lffw_vocab_loss_grad": ([ctypes.POINTER(VocabLossArgs), _vp], _i32),
+        "lffw_vocab_loss_error": ([ctypes.POINTER(_i32)], _i32),
         "lffw_chain_create": ([ctypes.POINTER(LinearArgs), _i32, ctypes.POINTER(_vp)], _i32),
         "lffw_chain_run": ([_vp, _vp], _i32),
         "lffw_chain_destroy": ([_vp], None),

@@ -24,8 +24,8 @@ ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 INCLUDE = ROOT / "include"
 LIBRARY = PACKAGE / "liblffw_b200.so"
-KERNEL_SOURCES = ("kernels.cu", "ptx.cuh", "launch.h")
-HOST_SOURCES = ("capi.cpp",)
+KERNEL_SOURCES = ("kernels.cu", "norm_train.cu", "vocab.cu", "ptx.cuh", "host_util.cuh", "launch.h")
+HOST_SOURCES = ("capi.cpp", "capi_training.cpp")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -62,7 +62,8 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
         "-Xcompiler", "-fPIC,-fvisibility=hidden",
         f"-I{INCLUDE}", f"-I{CSRC}",
         f'-DLFFW_BUNDLE_SHA256="{digest}"',
-        str(CSRC / "kernels.cu"), str(CSRC / "capi.cpp"),
+        "--threads", "0",
+        *(str(CSRC / name) for name in KERNEL_SOURCES + HOST_SOURCES if name.endswith((".cu", ".cpp"))),
         "-o", str(tmp),
     ]
     if verbose:

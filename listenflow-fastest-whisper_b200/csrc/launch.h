@@ -154,6 +154,57 @@ cudaError_t launch_fp16_gelu(const uint16_t *x, uint16_t *y, int64_t count, cuda
 cudaError_t launch_fp16_bias(const uint16_t *x, uint16_t bias, uint16_t *y, int64_t count,
                              cudaStream_t stream);
 
+// Operand types of the training kernels' launches (values of LFFW_DT_*).
+constexpr int kTypeFloat = 0;
+constexpr int kTypeHalf = 1;
+constexpr int kTypeBf16 = 7;
+
+// LayerNorm for training (fp16 or bf16 rows): forward fills sum_out, y and stats; backward
+// reads x (the summed rows), stats, dy and dsum and fills dx and/or dgamma and dbeta.
+struct LayerNormTrainLaunch {
+    int64_t rows, cols; // cols % 8 == 0, cols <= 4096
+    bool bf16;
+    const uint16_t *x, *residual;
+    uint16_t *sum_out, *y;
+    const float *gamma, *beta;
+    float eps;
+    float *stats;
+    const uint16_t *dy, *dsum;
+    uint16_t *dx;
+    float *dgamma, *dbeta;
+    void *workspace; // layer_norm_grad_workspace bytes, with dgamma
+};
+int64_t layer_norm_grad_workspace(int64_t rows, int64_t cols);
+cudaError_t launch_layer_norm_forward(const LayerNormTrainLaunch &p, cudaStream_t stream);
+cudaError_t launch_layer_norm_backward(const LayerNormTrainLaunch &p, cudaStream_t stream);
+
+// Losses over the vocabulary's logits x W^T, and their gradients.
+constexpr int kVocabMaxTargets = 256;
+struct VocabLossLaunch {
+    int64_t rows, width, vocab; // width % 8 == 0
+    bool bf16;
+    const void *x, *weight;
+    const void *labels; // one int32 or int64 per row, or
+    int label_bytes;
+    int64_t ignore_index;
+    int targets; // teacher entries per row (0: labels)
+    const int32_t *teacher_tokens;
+    const void *teacher_logits;
+    int teacher_type; // kType*
+    float temperature;
+    float *losses, *lse_out;    // forward
+    const float *lse_in, *dloss; // backward
+    void *dx, *dweight;
+    void *workspace;
+};
+int64_t vocab_loss_workspace(const VocabLossLaunch &p, bool backward);
+cudaError_t launch_vocab_loss(const VocabLossLaunch &p, cudaStream_t stream);
+cudaError_t launch_vocab_loss_grad(const VocabLossLaunch &p, cudaStream_t stream);
+// 1 when a token outside the vocabulary was met, 0 when none, -1 when it cannot be read.
+int read_and_clear_token_error();
+// The vocabulary kernels' bounded-wait word (see read_and_clear_device_error).
+cudaError_t read_and_clear_vocab_wait_error(int *site);
+
 cudaError_t read_and_clear_device_error(int *site);
 uint64_t launch_count();
 void count_launch();

@@ -11,8 +11,8 @@ namespace lffw {
 // Sticky per-device error word.  A bounded wait that gives up stores a site
 // code here; every other waiter polls it and abandons its loop so the grid
 // drains instead of hanging.  Host reads and clears it (lffw_device_error).
-// This header is included by exactly one translation unit (kernels.cu).
-__device__ int g_device_error = 0;
+// Each translation unit that includes this header holds a word of its own.
+static __device__ int g_device_error = 0;
 
 enum WaitSite : int {
     kSiteProducerEmpty = 1,

@@ -1,0 +1,1326 @@
+// sm_100a kernels of the vocabulary losses: cross entropy against tokens and distillation
+// from a teacher's top logits, over the logits z = x W^T of a token table W [V, d], forward
+// and backward, without holding the logits.
+//
+//   loss     lse_i = log sum_v exp(z_iv / T)
+//            loss_i = T^2 (sum_j t_ij log t_ij + S_i lse_i - sum_j t_ij z_{i,v_ij} / T)
+//            (one target with t = 1 and T = 1: lse_i - z_i,label)
+//   gradient G_iv = g_i T (exp(z_iv / T - lse_i) - t_iv),  dx = G W,  dW = G^T x
+//
+// Everything of size n x V runs through one tensor-core GEMM kernel in four forms:
+//   kStats   z tiles, reduced in the epilogue to a running maximum, a sum of exponentials and
+//            the targets' logits per row and column slice (merged by combine_kernel)
+//   kGrad    z tiles again, turned in the epilogue into a piece of G (16 bits, a range of
+//            vocabulary columns)
+//   kDx      that piece times its rows of W, summed over the pieces in fp32
+//   kDw      that piece transposed times x: its rows of dW
+// A piece of G is the only n x (part of V) tensor that ever exists.
+//
+// The work is bound by the tensor cores (2 n V d flops per form, four forms for a training
+// step: the logits are formed twice because they are not kept) once n exceeds a few hundred
+// rows; below that it is bound by streaming W (and writing dW).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+
+#include "host_util.cuh"
+#include "launch.h"
+#include "ptx.cuh"
+
+namespace lffw {
+
+namespace vocab {
+
+constexpr int kBM = 128;               // accumulator rows per CTA (TMEM lanes)
+constexpr int kBK = 64;                // K elements per stage: one 128-byte swizzle row
+constexpr int kUmmaK = 16;             // K of one kind::f16 MMA
+constexpr int kEpiWarps = 8;           // two per TMEM lane quarter, each with half of the tile's columns
+constexpr int kThreads = 64 + 32 * kEpiWarps; // warp 0 TMA, warp 1 MMA, warps 2-9 epilogue
+constexpr int kSub = 32;               // columns per epilogue step
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum Mode : int { kStats, kGrad, kDx, kDw };
+
+// A label or a teacher token outside the vocabulary was met (see lffw_vocab_loss_error).
+__device__ int g_token_error = 0;
+
+// kPair: a cluster of two CTAs computes a 256 x BN tile with cta_group::2 MMAs, each CTA
+// holding 128 rows of A, BN/2 rows of B and its half of the accumulator: per SM that halves
+// the B traffic, which a 128 x 256 tile of one CTA would need at 96 B/clk, above what the
+// L2 delivers.
+// Operand layouts in shared memory (128-byte swizzle either way):
+//   K-major   rows of 64 K elements, one TMA box
+//   MN-major  64 K rows of 64 MN elements per TMA box, boxes stacked along MN
+// x and W are K-major for z = x W^T; W is MN-major as B of G W; G and x are MN-major in G^T x.
+template <int BN, bool kPair, int MODE>
+struct Cfg {
+    static constexpr bool kAMn = MODE == kDw;
+    static constexpr bool kBMn = MODE == kDx || MODE == kDw;
+    static constexpr int kTileM = kPair ? 2 * kBM : kBM;
+    static constexpr int kBRows = kPair ? BN / 2 : BN; // B rows this CTA loads
+    static constexpr int kABytes = kBM * 128;
+    static constexpr int kBBytes = kBRows * 128;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kTxBytes = kPair ? 2 * kStageBytes : kStageBytes;
+    static constexpr int kStaging = MODE == kStats ? 0 : 4096; // per epilogue warp
+    static constexpr int kBarBytes = 256;
+    static constexpr int kBudget = 232448 - 1024;
+    static constexpr int kFit = (kBudget - kEpiWarps * kStaging - kBarBytes) / kStageBytes;
+    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kOffB = kStages * kABytes;
+    static constexpr int kOffStaging = kOffB + kStages * kBBytes;
+    static constexpr int kOffBar = kOffStaging + kEpiWarps * kStaging;
+    static constexpr int kSmemBytes = kOffBar + kBarBytes + 1024;
+    static constexpr int kTmemCols = 2 * BN; // two accumulators
+    static constexpr int kSlice = BN / 2;    // columns per epilogue warp
+    static constexpr uint32_t kIdesc = (1u << 4) | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u) |
+                                       (static_cast<uint32_t>(BN >> 3) << 17) |
+                                       (static_cast<uint32_t>(kTileM >> 4) << 24);
+    static_assert(BN == 128 || BN == 256, "tile width");
+    static_assert(kStages >= 4 && kSmemBytes <= 232448, "shared memory budget");
+    static_assert((2 * kStages + 5) * 8 + 8 <= kBarBytes, "barrier area");
+};
+
+struct Params {
+    int m, n;                    // rows and columns of the output
+    int m_tiles, n_tiles, num_tiles;
+    int num_kb, kb_per;          // K blocks, and how many of them one split sums
+    int n_first;                 // raster: 0 = M tiles fastest, 1 = N tiles fastest
+    uint32_t type_bits;          // instruction descriptor's operand types
+    // kStats and kGrad: row i is token i, column c is vocabulary entry col0 + c.
+    int col0;
+    float scale2;                // log2(e) / T
+    const void *labels;          // kStats, one target: int32 or int64 per row
+    int label_bytes;
+    const int32_t *t_index;      // sorted target columns [rows, targets] (INT_MAX: none)
+    const float *t_prob;
+    int targets;
+    float *part_max, *part_sum, *part_t; // [slices, rows]; part_t holds sum_j t_j z_j
+    float *label_z;              // kStats, one target: z of the label
+    const float *row_lse2, *row_gain; // kGrad: lse log2(e), and g T s
+    // kDx and kDw
+    const float *inv_gain;       // 1 / s
+    int accumulate;              // kDx: add to the fp32 planes
+};
+
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16)
+{
+    uint32_t r;
+    if (bf16)
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// fp32 pair a * b + c, each lane rounded once.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    uint64_t x, y, z, r;
+    memcpy(&x, &a, 8);
+    memcpy(&y, &b, 8);
+    memcpy(&z, &c, 8);
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    float2 f;
+    memcpy(&f, &r, 8);
+    return f;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    uint64_t x, y, r;
+    memcpy(&x, &a, 8);
+    memcpy(&y, &b, 8);
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    float2 f;
+    memcpy(&f, &r, 8);
+    return f;
+}
+
+// v[c] for a c that differs from lane to lane: a five-level selection, since registers
+// cannot be indexed.
+__device__ __forceinline__ float select32(const uint32_t (&v)[32], int c)
+{
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        w[i] = (c & 1) ? v[2 * i + 1] : v[2 * i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        w[i] = (c & 2) ? w[2 * i + 1] : w[2 * i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = (c & 4) ? w[2 * i + 1] : w[2 * i];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        w[i] = (c & 8) ? w[2 * i + 1] : w[2 * i];
+    return __uint_as_float((c & 16) ? w[1] : w[0]);
+}
+
+// First of the `count` sorted columns that is >= column.
+__device__ __forceinline__ int lower_bound(const int32_t *cols, int count, int column)
+{
+    int lo = 0, hi = count;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cols[mid] < column)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ int64_t load_label(const void *labels, int bytes, int64_t row)
+{
+    return bytes == 8 ? static_cast<const int64_t *>(labels)[row]
+                      : static_cast<int64_t>(static_cast<const int32_t *>(labels)[row]);
+}
+
+__device__ __forceinline__ void tma_store_add_3d(const CUtensorMap *map, uint32_t src, int32_t x, int32_t y, int32_t z)
+{
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+
+// Matrix descriptor of an MN-major operand: 64-wide boxes of 64 K rows stacked along MN
+// (8192 bytes apart, the leading offset), 8-row swizzle atoms stacked along K (1024 bytes,
+// the stride offset).
+__device__ __forceinline__ uint64_t desc_mn_boxes(uint32_t addr)
+{
+    uint64_t desc = static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
+    desc |= static_cast<uint64_t>(8192u >> 4) << 16;
+    desc |= static_cast<uint64_t>(1024u >> 4) << 32;
+    desc |= static_cast<uint64_t>(1u) << 46;
+    desc |= static_cast<uint64_t>(2u) << 61;
+    return desc;
+}
+
+// tm_a, tm_b: operands.  tm_out: G (kGrad), dW (kDw), dx itself or the fp32 planes (kDx).
+// Planes is the kDx form that writes fp32 planes instead of dx.
+template <int BN, bool kPair, int MODE, bool kBf16, bool kPlanes>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                const __grid_constant__ CUtensorMap tm_out, const Params p)
+{
+    using C = Cfg<BN, kPair, MODE>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    uint8_t *smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(smem);
+
+    const int warp = threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+    const uint32_t rank = kPair ? cluster_ctarank() : 0u;
+    const bool leader = rank == 0;
+    const int tile_step = kPair ? static_cast<int>(gridDim.x / 2) : static_cast<int>(gridDim.x);
+    const int tile_first = kPair ? static_cast<int>(blockIdx.x / 2) : static_cast<int>(blockIdx.x);
+    const uint32_t bar_full = sbase + C::kOffBar;
+    const uint32_t bar_empty = bar_full + 8 * C::kStages;
+    const uint32_t bar_acc_full = bar_empty + 8 * C::kStages;
+    const uint32_t bar_acc_empty = bar_acc_full + 16;
+    const uint32_t bar_drain = bar_acc_empty + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::kOffBar + (2 * C::kStages + 5) * 8);
+
+    struct Tile {
+        int m0, n0, kb0, kbn, split;
+    };
+    // Tile t: this CTA's first row, the tile's first column, and its K blocks.  A function of
+    // t alone: the producer, the MMA issuer and the epilogue agree.
+    auto tile_at = [&](int t) {
+        const int per_split = p.m_tiles * p.n_tiles;
+        const int split = t / per_split;
+        const int r = t - split * per_split;
+        const int mt = p.n_first ? r / p.n_tiles : r % p.m_tiles;
+        const int nt = p.n_first ? r % p.n_tiles : r / p.m_tiles;
+        Tile tile;
+        tile.m0 = mt * C::kTileM + static_cast<int>(rank) * kBM;
+        tile.n0 = nt * BN;
+        tile.split = split;
+        tile.kb0 = split * p.kb_per;
+        tile.kbn = min(p.kb_per, p.num_kb - tile.kb0);
+        return tile;
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(bar_acc_full + 8 * a, 1);
+            mbar_init(bar_acc_empty + 8 * a, kPair ? 2 * kEpiWarps : kEpiWarps);
+        }
+        mbar_init(bar_drain, 1);
+        fence_barrier_init();
+        prefetch_tensor_map(&tm_a);
+        prefetch_tensor_map(&tm_b);
+        if (MODE != kStats)
+            prefetch_tensor_map(&tm_out);
+    }
+    if (warp == 1) {
+        if (kPair) {
+            tmem_alloc_pair(smem_u32(tmem_slot), C::kTmemCols);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+            tmem_relinquish();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (kPair)
+        cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    // Everything this grid reads (the weights too: an optimizer may just have written them)
+    // and writes belongs to the previous kernel until it completes.  The next kernel may only
+    // then start, so that its own early reads cannot pass that one either.
+    griddepcontrol_wait();
+    griddepcontrol_launch_dependents();
+
+    if (warp == 0) {
+        // ---------------- TMA producer (one thread) ----------------
+        if (lane == 0) {
+            uint32_t used_mask = 0, parity_mask = 0;
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            auto load = [&](uint32_t dst, const CUtensorMap *map, uint32_t full, int x, int y) {
+                if (kPair)
+                    tma_load_2d_pair(dst, map, full, x, y);
+                else
+                    tma_load_2d(dst, map, full, x, y);
+            };
+            for (int t = tile_first; ok && t < p.num_tiles; t += tile_step) {
+                const Tile tile = tile_at(t);
+                const int b0 = tile.n0 + static_cast<int>(rank) * C::kBRows;
+                for (int i = 0; i < tile.kbn; ++i) {
+                    if (!mbar_wait(bar_empty + 8 * s, ph ^ 1u, kSiteProducerEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    const int k0 = (tile.kb0 + i) * kBK;
+                    if (leader)
+                        mbar_arrive_expect_tx(bar_full + 8 * s, C::kTxBytes);
+                    const uint32_t full = kPair ? map_to_rank(bar_full + 8 * s, 0) : bar_full + 8 * s;
+                    const uint32_t a = sbase + s * C::kABytes;
+                    const uint32_t b = sbase + C::kOffB + s * C::kBBytes;
+                    if (C::kAMn) {
+#pragma unroll
+                        for (int j = 0; j < kBM / 64; ++j)
+                            load(a + j * 8192, &tm_a, full, tile.m0 + 64 * j, k0);
+                    } else {
+                        load(a, &tm_a, full, k0, tile.m0);
+                    }
+                    if (C::kBMn) {
+#pragma unroll
+                        for (int j = 0; j < C::kBRows / 64; ++j)
+                            load(b + j * 8192, &tm_b, full, b0 + 64 * j, k0);
+                    } else {
+                        load(b, &tm_b, full, k0, b0);
+                    }
+                    used_mask |= 1u << s;
+                    parity_mask = (parity_mask & ~(1u << s)) | (ph << s);
+                    if (++s == C::kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            // Every issued load must land before shared memory is released.  In a pair the
+            // leader's full barriers count both CTAs' loads.
+            if (leader)
+                for (int i = 0; i < C::kStages; ++i)
+                    if (used_mask & (1u << i)) {
+                        const uint32_t par = (parity_mask >> i) & 1u;
+                        for (int tries = 0; tries < (1 << 22) && !mbar_try_wait(bar_full + 8 * i, par); ++tries) {
+                        }
+                    }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (one thread of the leader) ----------------
+        if (lane == 0 && leader) {
+            const uint32_t idesc = C::kIdesc | p.type_bits;
+            int s = 0;
+            uint32_t ph = 0;
+            int local = 0;
+            bool ok = true;
+            for (int t = tile_first; ok && t < p.num_tiles; t += tile_step) {
+                const Tile tile = tile_at(t);
+                if (tile.kbn <= 0)
+                    continue;
+                const uint32_t a = local & 1;
+                const uint32_t acc_ph = (local >> 1) & 1;
+                ++local;
+                if (!mbar_wait(bar_acc_empty + 8 * a, acc_ph ^ 1u, kSiteMmaAccEmpty)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + a * BN;
+                for (int i = 0; i < tile.kbn; ++i) {
+                    if (!mbar_wait(bar_full + 8 * s, ph, kSiteMmaFull)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a_addr = sbase + s * C::kABytes;
+                    const uint32_t b_addr = sbase + C::kOffB + s * C::kBBytes;
+#pragma unroll
+                    for (int k = 0; k < kBK / kUmmaK; ++k) {
+                        // 16 K elements: 32 bytes of a K-major row, or two 8-row atoms.
+                        const uint64_t da =
+                            C::kAMn ? desc_mn_boxes(a_addr + k * 2048) : smem_desc_k_sw128(a_addr + k * 32);
+                        const uint64_t db =
+                            C::kBMn ? desc_mn_boxes(b_addr + k * 2048) : smem_desc_k_sw128(b_addr + k * 32);
+                        if (kPair)
+                            mma_f16_pair(d_tmem, da, db, idesc, (i | k) != 0);
+                        else
+                            mma_f16(d_tmem, da, db, idesc, (i | k) != 0);
+                    }
+                    if (kPair)
+                        mma_commit_pair_both(bar_empty + 8 * s);
+                    else
+                        mma_commit(bar_empty + 8 * s);
+                    if (++s == C::kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+                if (ok) {
+                    if (kPair)
+                        mma_commit_pair_both(bar_acc_full + 8 * a);
+                    else
+                        mma_commit(bar_acc_full + 8 * a);
+                }
+            }
+            // Drain: all MMAs issued by this thread complete before TMEM is freed.
+            if (kPair)
+                mma_commit_pair_local(bar_drain);
+            else
+                mma_commit(bar_drain);
+            for (int tries = 0; tries < (1 << 22) && !mbar_try_wait(bar_drain, 0); ++tries) {
+            }
+        }
+    } else {
+        // ---------------- Epilogue: 8 independent warps, one row per lane ----------------
+        const int ew = warp - 2;
+        const int quarter = warp & 3;
+        const int half = ew >> 2; // this warp's half of the tile's columns
+        const uint32_t acc_empty = kPair ? map_to_rank(bar_acc_empty, 0) : bar_acc_empty;
+        uint8_t *staging = smem + C::kOffStaging + ew * C::kStaging;
+        const uint32_t staging_s = smem_u32(staging);
+        const float inv_gain = MODE == kDw || (MODE == kDx && !kPlanes) ? *p.inv_gain : 1.0f;
+        int local = 0, stores = 0;
+        for (int t = tile_first; t < p.num_tiles; t += tile_step) {
+            const Tile tile = tile_at(t);
+            if (tile.kbn <= 0)
+                continue;
+            const uint32_t a = local & 1;
+            const uint32_t acc_ph = (local >> 1) & 1;
+            ++local;
+            const int row0 = tile.m0 + quarter * 32;
+            const int row = row0 + lane;
+            const int col0 = tile.n0 + half * C::kSlice;
+            // Rows and columns of this warp that exist.
+            const int width = row0 < p.m ? min(C::kSlice, p.n - col0) : 0;
+            const int subs = width > 0 ? (width + kSub - 1) / kSub : 0;
+
+            // The row's next target column (relative to the piece), found while the MMAs run.
+            int next = INT_MAX, entry = 0;
+            const int32_t *row_cols = nullptr;
+            float lse2 = 0.0f, gain = 0.0f;
+            if ((MODE == kStats || MODE == kGrad) && row < p.m && subs > 0) {
+                if (p.t_index) {
+                    row_cols = p.t_index + static_cast<size_t>(row) * p.targets;
+                    entry = lower_bound(row_cols, p.targets, p.col0 + col0);
+                    if (entry < p.targets)
+                        next = row_cols[entry] - p.col0; // INT_MAX - col0 never falls in a tile
+                } else {
+                    const int64_t label = load_label(p.labels, p.label_bytes, row);
+                    if (label >= col0 && label < p.n)
+                        next = static_cast<int>(label);
+                }
+                if (MODE == kGrad) {
+                    lse2 = p.row_lse2[row];
+                    gain = p.row_gain[row];
+                }
+            }
+            float run_max = -INFINITY, run_sum = 0.0f, run_t = 0.0f;
+
+            const bool ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_full + 8 * a, acc_ph, kSiteEpilogueAccFull));
+            if (!ok)
+                break;
+            tc_fence_after();
+            const uint32_t t_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + a * BN + half * C::kSlice;
+#pragma unroll 1
+            for (int sub = 0; sub < subs; ++sub) {
+                const int c0 = col0 + sub * kSub;
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(t_base + sub * kSub, v);
+                tmem_wait_ld();
+                if (sub == subs - 1) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (kPair)
+                            mbar_arrive_cluster(acc_empty + 8 * a);
+                        else
+                            mbar_arrive(acc_empty + 8 * a);
+                    }
+                }
+                if (MODE == kStats) {
+                    // Running maximum and sum of exp2(scale2 z - maximum).
+                    if (p.n - c0 < kSub) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (c0 + i >= p.n)
+                                v[i] = 0xff800000u; // columns past the vocabulary: -infinity
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            mx[j] = fmaxf(mx[j], fmaxf(__uint_as_float(v[i + 2 * j]), __uint_as_float(v[i + 2 * j + 1])));
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2;
+                    const float next_max = fmaxf(run_max, top);
+                    const float2 ref = make_float2(-next_max, -next_max);
+                    const float2 sc = make_float2(p.scale2, p.scale2);
+                    float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 e =
+                            fma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc, ref);
+                        acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], make_float2(exp2_approx(e.x), exp2_approx(e.y)));
+                    }
+                    acc[0] = add2(acc[0], acc[1]);
+                    run_sum = fmaf(run_sum, exp2_approx(run_max - next_max), acc[0].x + acc[0].y);
+                    run_max = next_max;
+                    // Targets of this step: rare, so one uniform test in the common case.
+                    while (__any_sync(0xffffffffu, next < c0 + kSub)) {
+                        if (next < c0 + kSub) {
+                            const float z = select32(v, next - c0);
+                            if (p.t_index) {
+                                run_t = fmaf(p.t_prob[static_cast<size_t>(row) * p.targets + entry], z, run_t);
+                                ++entry;
+                                next = entry < p.targets ? row_cols[entry] - p.col0 : INT_MAX;
+                            } else {
+                                p.label_z[row] = z;
+                                next = INT_MAX;
+                            }
+                        }
+                    }
+                    continue;
+                }
+                uint32_t h[16];
+                float f[32];
+                if (MODE == kGrad) {
+                    const float2 ref = make_float2(-lse2, -lse2);
+                    const float2 sc = make_float2(p.scale2, p.scale2);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 e =
+                            fma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc, ref);
+                        f[i] = exp2_approx(e.x) * gain;
+                        f[i + 1] = exp2_approx(e.y) * gain;
+                    }
+                    while (__any_sync(0xffffffffu, next < c0 + kSub)) {
+                        if (next < c0 + kSub) {
+                            const int c = next - c0;
+                            const float d = gain * p.t_prob[static_cast<size_t>(row) * p.targets + entry];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                f[i] = i == c ? f[i] - d : f[i];
+                            ++entry;
+                            next = entry < p.targets ? row_cols[entry] - p.col0 : INT_MAX;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        f[i] = __uint_as_float(v[i]) * inv_gain;
+                }
+                if (MODE == kDx && kPlanes) {
+                    // 32 rows x 128 B of fp32, 128-byte swizzle: chunk j of row r at j ^ (r & 7).
+                    if (lane == 0)
+                        bulk_wait_group_read0();
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        *reinterpret_cast<float4 *>(staging + lane * 128 + ((j ^ (lane & 7)) * 16)) =
+                            make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (p.accumulate)
+                            tma_store_add_3d(&tm_out, staging_s, c0, row0, tile.split);
+                        else
+                            tma_store_3d(&tm_out, staging_s, c0, row0, tile.split);
+                        bulk_commit_group();
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        h[i] = pack16(f[2 * i], f[2 * i + 1], kBf16);
+                    // Two buffers of 32 rows x 64 B, 64-byte swizzle: chunk j of row r at
+                    // j ^ ((r >> 1) & 3).  All but the newest store have read theirs.
+                    const uint32_t buf = (stores & 1) * 2048u;
+                    ++stores;
+                    if (lane == 0)
+                        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *reinterpret_cast<uint4 *>(staging + buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) =
+                            make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tm_out, staging_s + buf, c0, row0);
+                        bulk_commit_group();
+                    }
+                }
+            }
+            if (subs == 0) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (kPair)
+                        mbar_arrive_cluster(acc_empty + 8 * a);
+                    else
+                        mbar_arrive(acc_empty + 8 * a);
+                }
+            }
+            if (MODE == kStats && subs > 0 && row < p.m) {
+                const size_t at = static_cast<size_t>(col0 / C::kSlice) * p.m + row;
+                p.part_max[at] = run_max;
+                p.part_sum[at] = run_sum;
+                if (p.part_t)
+                    p.part_t[at] = run_t;
+            }
+        }
+        if (MODE != kStats && lane == 0)
+            bulk_wait_group0();
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (kPair)
+        cluster_sync(); // neither CTA leaves while its peer may still touch its barriers or TMEM
+    if (warp == 1) {
+        tc_fence_after();
+        if (kPair)
+            tmem_dealloc_pair(tmem_base, C::kTmemCols);
+        else
+            tmem_dealloc(tmem_base, C::kTmemCols);
+    }
+}
+
+// ---- targets ------------------------------------------------------------------
+
+__device__ __forceinline__ float load_float(const void *p, int dtype, size_t i)
+{
+    if (dtype == kTypeFloat)
+        return static_cast<const float *>(p)[i];
+    if (dtype == kTypeBf16)
+        return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+    return __half2float(static_cast<const __half *>(p)[i]);
+}
+
+constexpr int kPrepWarps = 8;
+constexpr int kPerLane = kVocabMaxTargets / 32;
+
+struct Targets {
+    int rows, vocab, count;
+    const int32_t *tokens;
+    const void *logits;
+    int logit_type;
+    float inv_temperature;
+    int32_t *index; // sorted [rows, count]
+    float *prob;
+};
+
+// One warp lays out one row's teacher entries: the softmax of the logits of the valid ones
+// (token in the vocabulary, logit not -infinity) and their columns in ascending order, by
+// ranks (stable, so equal tokens keep their order), the rest INT_MAX.  Returns whether the
+// row has any, with (negative entropy, sum) of its probabilities in 64 bits: the loss is a
+// difference of terms near log(V), so it is formed from unrounded ones.
+__device__ __forceinline__ bool sort_targets(const Targets &t, int row, int lane, int32_t *cols, double &entropy,
+                                             double &total)
+{
+    const size_t base = static_cast<size_t>(row) * t.count;
+    int32_t col[kPerLane];
+    float z[kPerLane];
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+        const int j = lane + 32 * i;
+        col[i] = INT_MAX;
+        z[i] = -INFINITY;
+        if (j < t.count) {
+            const int32_t token = t.tokens[base + j];
+            if (token >= t.vocab)
+                g_token_error = 1;
+            if (token >= 0 && token < t.vocab) {
+                z[i] = load_float(t.logits, t.logit_type, base + j) * t.inv_temperature;
+                col[i] = z[i] == -INFINITY ? INT_MAX : token;
+            }
+            cols[j] = col[i];
+        }
+        top = fmaxf(top, z[i]);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float e[kPerLane], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+        e[i] = col[i] == INT_MAX ? 0.0f : exp2f((z[i] - top) * kLog2e);
+        sum += e[i];
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncwarp();
+    const bool any = __any_sync(0xffffffffu, [&] {
+        bool has = false;
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i)
+            has |= col[i] != INT_MAX;
+        return has;
+    }());
+    entropy = 0.0;
+    total = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+        const int j = lane + 32 * i;
+        if (j < t.count) {
+            int rank = 0;
+            for (int o = 0; o < t.count; ++o)
+                rank += cols[o] < col[i] || (cols[o] == col[i] && o < j);
+            const float prob = any ? e[i] / sum : 0.0f;
+            t.index[base + rank] = col[i];
+            t.prob[base + rank] = prob;
+            if (col[i] != INT_MAX) {
+                entropy += static_cast<double>(prob) * (static_cast<double>(z[i]) - static_cast<double>(top));
+                total += prob;
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        entropy += __shfl_xor_sync(0xffffffffu, entropy, o);
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    if (any)
+        entropy -= total * log(static_cast<double>(sum));
+    __syncwarp();
+    return any;
+}
+
+// Forward of the distillation: sorted targets, and (entropy, sum) per row.
+__global__ void __launch_bounds__(32 * kPrepWarps) targets_kernel(const Targets t, double2 *row_terms)
+{
+    __shared__ int32_t cols[kPrepWarps][kVocabMaxTargets];
+    griddepcontrol_wait();
+    griddepcontrol_launch_dependents();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    for (int row = blockIdx.x * kPrepWarps + warp; row < t.rows; row += gridDim.x * kPrepWarps) {
+        double entropy, total;
+        sort_targets(t, row, lane, cols[warp], entropy, total);
+        if (lane == 0)
+            row_terms[row] = make_double2(entropy, total);
+    }
+}
+
+struct Prepare {
+    Targets t;            // distillation (t.tokens set), or
+    const void *labels;   // one label per row
+    int label_bytes;
+    int64_t ignore_index;
+    float temperature;
+    int width;            // elements per row of x, a multiple of 8
+    const void *x;
+    void *x_masked;
+    const float *lse, *grad;
+    float *row_lse2, *row_gain, *inv_gain;
+};
+
+// Backward's first step: per row its targets, lse and gain g T s, and a copy of x whose rows
+// without a target are zero, so that whatever those hold (NaN included) reaches neither G nor
+// dW.  s = 2^(13 - exponent of max |g T|) puts |g T s| in [2^13, 2^14): with |p - t| <= 1, G
+// then fits fp16 and keeps 11 bits down to p = 2^-28.
+__global__ void __launch_bounds__(32 * kPrepWarps) prepare_kernel(const Prepare p)
+{
+    __shared__ int32_t cols[kPrepWarps][kVocabMaxTargets];
+    __shared__ float warp_max[kPrepWarps];
+    griddepcontrol_wait();
+    griddepcontrol_launch_dependents();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    // The largest finite |g|: every block reads all of them (a few KB).
+    float top = 0.0f;
+    for (int i = threadIdx.x; i < p.t.rows; i += blockDim.x) {
+        const float g = fabsf(p.grad[i]);
+        top = fmaxf(top, g < INFINITY ? g : 0.0f);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0)
+        warp_max[warp] = top;
+    __syncthreads();
+    top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPrepWarps; ++i)
+        top = fmaxf(top, warp_max[i]);
+    top *= p.temperature;
+    const int exponent = top > 0.0f && top < INFINITY ? min(max(ilogbf(top), -100), 100) : 13;
+    const float s = ldexpf(1.0f, 13 - exponent);
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        *p.inv_gain = ldexpf(1.0f, exponent - 13);
+
+    for (int row = blockIdx.x * kPrepWarps + warp; row < p.t.rows; row += gridDim.x * kPrepWarps) {
+        bool any;
+        if (p.t.tokens) {
+            double entropy, total;
+            any = sort_targets(p.t, row, lane, cols[warp], entropy, total);
+        } else {
+            const int64_t label = load_label(p.labels, p.label_bytes, row);
+            any = label != p.ignore_index && label >= 0 && label < p.t.vocab;
+            if (lane == 0) {
+                if (!any && label != p.ignore_index)
+                    g_token_error = 1;
+                p.t.index[row] = any ? static_cast<int32_t>(label) : INT_MAX;
+                p.t.prob[row] = 1.0f;
+            }
+        }
+        if (lane == 0) {
+            p.row_lse2[row] = any ? p.lse[row] * kLog2e : 0.0f;
+            p.row_gain[row] = any ? p.grad[row] * p.temperature * s : 0.0f;
+        }
+        const size_t base = static_cast<size_t>(row) * (p.width / 8);
+        const uint4 *src = static_cast<const uint4 *>(p.x) + base;
+        uint4 *dst = static_cast<uint4 *>(p.x_masked) + base;
+        for (int i = lane; i < p.width / 8; i += 32)
+            dst[i] = any ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+
+// ---- forward's last step ---------------------------------------------------------
+
+struct Combine {
+    int rows, slices, vocab;
+    const float *part_max, *part_sum, *part_t;
+    const float *label_z;
+    const void *labels;
+    int label_bytes;
+    int64_t ignore_index;
+    const double2 *row_terms;
+    float temperature;
+    float *losses, *lse;
+};
+
+constexpr int kCombineGroups = 32;
+
+// Merges the slices' maxima and sums (and target products) of 32 rows per block, lane = row,
+// in a fixed order; the loss is formed in 64 bits because it is a difference of terms near
+// log(V).
+__global__ void __launch_bounds__(32 * kCombineGroups) combine_kernel(const Combine p)
+{
+    __shared__ float s_max[kCombineGroups][32], s_sum[kCombineGroups][32];
+    __shared__ double s_t[kCombineGroups][32];
+    griddepcontrol_wait();
+    griddepcontrol_launch_dependents();
+    const int group = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int row = blockIdx.x * 32 + lane;
+    float mx = -INFINITY, sum = 0.0f;
+    double target = 0.0;
+    if (row < p.rows) {
+#pragma unroll 4
+        for (int i = group; i < p.slices; i += kCombineGroups) {
+            const size_t at = static_cast<size_t>(i) * p.rows + row;
+            const float m = p.part_max[at], s = p.part_sum[at];
+            if (p.part_t)
+                target += p.part_t[at];
+            const float next = fmaxf(mx, m);
+            sum = fmaf(sum, exp2f(mx - next), s * exp2f(m - next));
+            mx = next;
+        }
+    }
+    s_max[group][lane] = mx;
+    s_sum[group][lane] = sum;
+    s_t[group][lane] = target;
+    __syncthreads();
+    if (group != 0 || row >= p.rows)
+        return;
+    for (int i = 1; i < kCombineGroups && i < p.slices; ++i) {
+        const float m = s_max[i][lane];
+        const float next = fmaxf(mx, m);
+        sum = fmaf(sum, exp2f(mx - next), s_sum[i][lane] * exp2f(m - next));
+        mx = next;
+        target += s_t[i][lane];
+    }
+    const double lse = static_cast<double>(mx) * 0.69314718055994530942 + log(static_cast<double>(sum));
+    p.lse[row] = static_cast<float>(lse);
+    double loss = 0.0;
+    if (p.row_terms) {
+        const double2 terms = p.row_terms[row];
+        if (terms.y != 0.0) {
+            const double temperature = p.temperature;
+            loss = temperature * temperature * (terms.x + terms.y * lse - target / temperature);
+        }
+    } else {
+        const int64_t label = load_label(p.labels, p.label_bytes, row);
+        if (label != p.ignore_index) {
+            if (label >= 0 && label < p.vocab)
+                loss = lse - static_cast<double>(p.label_z[row]);
+            else
+                g_token_error = 1;
+        }
+    }
+    p.losses[row] = static_cast<float>(loss);
+}
+
+// dx = sum of the fp32 planes (one per K split), in order, times 1 / s: eight elements per thread.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) planes_kernel(const float *planes, int count, size_t elements,
+                                                     const float *inv_gain, uint4 *dx)
+{
+    griddepcontrol_wait();
+    griddepcontrol_launch_dependents();
+    const float inv = *inv_gain;
+    for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < elements / 8;
+         i += static_cast<size_t>(gridDim.x) * blockDim.x) {
+        float f[8] = {};
+        for (int s = 0; s < count; ++s) {
+            const float4 *src = reinterpret_cast<const float4 *>(planes + s * elements) + 2 * i;
+            const float4 lo = src[0], hi = src[1];
+            f[0] += lo.x, f[1] += lo.y, f[2] += lo.z, f[3] += lo.w;
+            f[4] += hi.x, f[5] += hi.y, f[6] += hi.z, f[7] += hi.w;
+        }
+        dx[i] = make_uint4(pack16(f[0] * inv, f[1] * inv, kBf16), pack16(f[2] * inv, f[3] * inv, kBf16),
+                           pack16(f[4] * inv, f[5] * inv, kBf16), pack16(f[6] * inv, f[7] * inv, kBf16));
+    }
+}
+
+} // namespace vocab
+
+// ---- host ---------------------------------------------------------------------------
+
+namespace {
+
+using namespace vocab;
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Up to this many rows one CTA per 128 x 128 tile of z is used instead of a pair per
+// 256 x 256: the rows fit one accumulator, W is streamed once, and narrow tiles spread it
+// over the SMs evenly.
+constexpr int64_t kSingleRows = 128;
+
+// Bytes of one piece of G.
+constexpr int64_t kPieceBytes = int64_t{256} << 20;
+
+struct Arena {
+    uint8_t *base;
+    int64_t used = 0;
+    template <class T>
+    T *take(int64_t count)
+    {
+        T *at = reinterpret_cast<T *>(base + used);
+        used += round_up(count * static_cast<int64_t>(sizeof(T)), 256);
+        return at;
+    }
+};
+
+struct ForwardPlan {
+    bool single;
+    int slice;
+    int64_t slices;
+    float *part_max, *part_sum, *part_t, *label_z, *t_prob;
+    int32_t *t_index;
+    double2 *row_terms;
+    int64_t bytes;
+};
+
+ForwardPlan plan_forward(const VocabLossLaunch &L, void *workspace)
+{
+    ForwardPlan f{};
+    Arena arena{static_cast<uint8_t *>(workspace)};
+    f.single = L.rows <= kSingleRows;
+    f.slice = f.single ? 64 : 128;
+    f.slices = ceil_div(L.vocab, f.slice);
+    f.part_max = arena.take<float>(f.slices * L.rows);
+    f.part_sum = arena.take<float>(f.slices * L.rows);
+    if (L.targets > 0) {
+        f.part_t = arena.take<float>(f.slices * L.rows);
+        f.t_index = arena.take<int32_t>(L.rows * L.targets);
+        f.t_prob = arena.take<float>(L.rows * L.targets);
+        f.row_terms = arena.take<double2>(L.rows);
+    } else {
+        f.label_z = arena.take<float>(L.rows);
+    }
+    f.bytes = arena.used;
+    return f;
+}
+
+struct BackwardPlan {
+    bool single;
+    int targets;
+    int64_t piece, pieces;   // vocabulary columns per piece of G
+    int64_t ldg;             // elements per row of a piece
+    int dx_bn, dw_bn;
+    int64_t splits;          // K splits of dx
+    bool planes;
+    float *row_lse2, *row_gain, *inv_gain, *t_prob, *dx_planes;
+    int32_t *t_index;
+    void *x_masked, *g;
+    int64_t bytes;
+};
+
+// A 128-wide tile where it saves a whole half tile of padding.
+int tile_width(int64_t columns) { return columns % 256 != 0 && columns % 256 <= 128 ? 128 : 256; }
+
+BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
+{
+    BackwardPlan b{};
+    Arena arena{static_cast<uint8_t *>(workspace)};
+    b.single = L.rows <= kSingleRows;
+    b.targets = L.targets > 0 ? L.targets : 1;
+    const int64_t most = std::max<int64_t>(256, kPieceBytes / 2 / L.rows / 256 * 256);
+    b.pieces = ceil_div(L.vocab, most);
+    b.piece = std::min(L.vocab, round_up(ceil_div(L.vocab, b.pieces), 256));
+    b.pieces = ceil_div(L.vocab, b.piece);
+    b.ldg = round_up(b.piece, 64);
+    b.dx_bn = b.single ? 128 : tile_width(L.width);
+    b.dw_bn = tile_width(L.width);
+    const int64_t units = b.single ? sm_count() : sm_count() / 2;
+    const int64_t tiles = ceil_div(L.rows, b.single ? kBM : 2 * kBM) * ceil_div(L.width, b.dx_bn);
+    const int64_t kbs = ceil_div(b.piece, kBK);
+    const int64_t want = std::max<int64_t>(1, std::min(units / std::max<int64_t>(tiles, 1), kbs / 4));
+    b.splits = ceil_div(kbs, ceil_div(kbs, want));
+    b.planes = b.splits > 1 || b.pieces > 1;
+    b.row_lse2 = arena.take<float>(L.rows);
+    b.row_gain = arena.take<float>(L.rows);
+    b.inv_gain = arena.take<float>(1);
+    b.t_index = arena.take<int32_t>(L.rows * b.targets);
+    b.t_prob = arena.take<float>(L.rows * b.targets);
+    b.x_masked = arena.take<uint16_t>(L.rows * L.width);
+    b.g = arena.take<uint16_t>(L.rows * b.ldg);
+    if (L.dx && b.planes)
+        b.dx_planes = arena.take<float>(b.splits * L.rows * L.width);
+    b.bytes = arena.used;
+    return b;
+}
+
+// fp16/bf16 operand [rows, cols], rows `ld` elements apart.
+bool map16(CUtensorMap *map, bool bf16, const void *base, int64_t rows, int64_t cols, int64_t ld, int box_cols,
+           int box_rows, CUtensorMapSwizzle swizzle)
+{
+    return make_map_ld(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, rows,
+                       cols, ld, static_cast<uint32_t>(box_cols), static_cast<uint32_t>(box_rows), swizzle);
+}
+
+// An operand of a GEMM: K-major ([mn, k] in memory) or MN-major ([k, mn]).
+bool operand_map(CUtensorMap *map, bool bf16, bool mn_major, const void *base, int64_t rows, int64_t cols, int64_t ld,
+                 int mn_rows)
+{
+    return mn_major ? map16(map, bf16, base, rows, cols, ld, 64, kBK, CU_TENSOR_MAP_SWIZZLE_128B)
+                    : map16(map, bf16, base, rows, cols, ld, kBK, mn_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int BN, bool kPair, int MODE, bool kBf16, bool kPlanes>
+cudaError_t launch_one(const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &out, Params p,
+                       cudaStream_t stream)
+{
+    using C = Cfg<BN, kPair, MODE>;
+    auto kernel = gemm_kernel<BN, kPair, MODE, kBf16, kPlanes>;
+    static std::atomic<bool> opted[kMaxDevices];
+    const int device = current_device();
+    if (!opted[device].load(std::memory_order_acquire)) {
+        const cudaError_t err =
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+        if (err != cudaSuccess)
+            return err;
+        opted[device].store(true, std::memory_order_release);
+    }
+    p.m_tiles = static_cast<int>(ceil_div(p.m, C::kTileM));
+    p.n_tiles = static_cast<int>(ceil_div(p.n, BN));
+    const int64_t splits = ceil_div(p.num_kb, p.kb_per);
+    p.num_tiles = static_cast<int>(splits * p.m_tiles * p.n_tiles);
+    p.type_bits = kBf16 ? (1u << 7) | (1u << 10) : 0u;
+    const int units = kPair ? sm_count() / 2 : sm_count();
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(std::min(p.num_tiles, units) * (kPair ? 2 : 1)));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = C::kSmemBytes;
+    config.stream = stream;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    config.numAttrs = 1;
+    if (kPair) {
+        attrs[1].id = cudaLaunchAttributeClusterDimension;
+        attrs[1].val.clusterDim.x = 2;
+        attrs[1].val.clusterDim.y = 1;
+        attrs[1].val.clusterDim.z = 1;
+        config.numAttrs = 2;
+    }
+    config.attrs = attrs;
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, a, b, out, p);
+    count_launch();
+    return err != cudaSuccess ? err : cudaGetLastError();
+}
+
+// z tiles: x [rows, width] times columns [col0, col0 + cols) of W^T.
+template <int MODE, bool kBf16>
+cudaError_t launch_logits(const VocabLossLaunch &L, const void *x, int64_t col0, int64_t cols, bool single,
+                          const CUtensorMap &out, Params p, cudaStream_t stream)
+{
+    CUtensorMap a, b;
+    const uint16_t *w = static_cast<const uint16_t *>(L.weight) + col0 * L.width;
+    if (!operand_map(&a, kBf16, false, x, L.rows, L.width, L.width, kBM) ||
+        !operand_map(&b, kBf16, false, w, cols, L.width, L.width, 128))
+        return cudaErrorInvalidValue;
+    p.m = static_cast<int>(L.rows);
+    p.n = static_cast<int>(cols);
+    p.col0 = static_cast<int>(col0);
+    p.num_kb = p.kb_per = static_cast<int>(ceil_div(L.width, kBK));
+    p.scale2 = static_cast<float>(1.4426950408889634 / static_cast<double>(L.temperature));
+    return single ? launch_one<128, false, MODE, kBf16, false>(a, b, out, p, stream)
+                  : launch_one<256, true, MODE, kBf16, false>(a, b, out, p, stream);
+}
+
+template <bool kBf16>
+cudaError_t run_forward(const VocabLossLaunch &L, cudaStream_t stream)
+{
+    const ForwardPlan f = plan_forward(L, L.workspace);
+    cudaError_t err;
+    Params p{};
+    if (L.targets > 0) {
+        Targets t{};
+        t.rows = static_cast<int>(L.rows);
+        t.vocab = static_cast<int>(L.vocab);
+        t.count = L.targets;
+        t.tokens = L.teacher_tokens;
+        t.logits = L.teacher_logits;
+        t.logit_type = L.teacher_type;
+        t.inv_temperature = 1.0f / L.temperature;
+        t.index = f.t_index;
+        t.prob = f.t_prob;
+        const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, kPrepWarps), 8 * sm_count());
+        err = launch_pdl(targets_kernel, dim3(static_cast<unsigned>(blocks)), dim3(32 * kPrepWarps), stream, t,
+                         f.row_terms);
+        if (err != cudaSuccess)
+            return err;
+        p.t_index = f.t_index;
+        p.t_prob = f.t_prob;
+        p.targets = L.targets;
+    }
+    p.labels = L.labels;
+    p.label_bytes = L.label_bytes;
+    p.part_max = f.part_max;
+    p.part_sum = f.part_sum;
+    p.part_t = f.part_t;
+    p.label_z = f.label_z;
+    err = launch_logits<kStats, kBf16>(L, L.x, 0, L.vocab, f.single, CUtensorMap{}, p, stream);
+    if (err != cudaSuccess)
+        return err;
+    Combine c{};
+    c.rows = static_cast<int>(L.rows);
+    c.slices = static_cast<int>(f.slices);
+    c.vocab = static_cast<int>(L.vocab);
+    c.part_max = f.part_max;
+    c.part_sum = f.part_sum;
+    c.part_t = f.part_t;
+    c.label_z = f.label_z;
+    c.labels = L.labels;
+    c.label_bytes = L.label_bytes;
+    c.ignore_index = L.ignore_index;
+    c.row_terms = f.row_terms;
+    c.temperature = L.temperature;
+    c.losses = L.losses;
+    c.lse = L.lse_out;
+    return launch_pdl(combine_kernel, dim3(static_cast<unsigned>(ceil_div(L.rows, 32))), dim3(32 * kCombineGroups),
+                      stream, c);
+}
+
+template <bool kBf16>
+cudaError_t launch_dx(const VocabLossLaunch &L, const BackwardPlan &b, int64_t col0, int64_t cols, bool first,
+                      cudaStream_t stream)
+{
+    CUtensorMap ma, mb, out;
+    const uint16_t *w = static_cast<const uint16_t *>(L.weight) + col0 * L.width;
+    if (!operand_map(&ma, kBf16, false, b.g, L.rows, cols, b.ldg, kBM) ||
+        !operand_map(&mb, kBf16, true, w, cols, L.width, L.width, 0))
+        return cudaErrorInvalidValue;
+    if (b.planes) {
+        const int64_t dims[3] = {L.width, L.rows, b.splits};
+        const int64_t strides[2] = {L.width * 4, L.rows * L.width * 4};
+        const uint32_t box[3] = {kSub, 32u, 1u};
+        if (!make_map_nd(&out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, b.dx_planes, dims, strides, box,
+                         CU_TENSOR_MAP_SWIZZLE_128B))
+            return cudaErrorInvalidValue;
+    } else if (!map16(&out, kBf16, L.dx, L.rows, L.width, L.width, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
+        return cudaErrorInvalidValue;
+    }
+    Params p{};
+    p.m = static_cast<int>(L.rows);
+    p.n = static_cast<int>(L.width);
+    p.num_kb = static_cast<int>(ceil_div(cols, kBK));
+    p.kb_per = static_cast<int>(ceil_div(ceil_div(b.piece, kBK), b.splits));
+    p.n_first = 1;
+    p.inv_gain = b.inv_gain;
+    p.accumulate = first ? 0 : 1;
+    if (b.planes) {
+        if (b.single)
+            return launch_one<128, false, kDx, kBf16, true>(ma, mb, out, p, stream);
+        return b.dx_bn == 128 ? launch_one<128, true, kDx, kBf16, true>(ma, mb, out, p, stream)
+                              : launch_one<256, true, kDx, kBf16, true>(ma, mb, out, p, stream);
+    }
+    if (b.single)
+        return launch_one<128, false, kDx, kBf16, false>(ma, mb, out, p, stream);
+    return b.dx_bn == 128 ? launch_one<128, true, kDx, kBf16, false>(ma, mb, out, p, stream)
+                          : launch_one<256, true, kDx, kBf16, false>(ma, mb, out, p, stream);
+}
+
+template <bool kBf16>
+cudaError_t launch_dw(const VocabLossLaunch &L, const BackwardPlan &b, int64_t col0, int64_t cols,
+                      cudaStream_t stream)
+{
+    CUtensorMap ma, mb, out;
+    uint16_t *dw = static_cast<uint16_t *>(L.dweight) + col0 * L.width;
+    if (!operand_map(&ma, kBf16, true, b.g, L.rows, cols, b.ldg, 0) ||
+        !operand_map(&mb, kBf16, true, b.x_masked, L.rows, L.width, L.width, 0) ||
+        !map16(&out, kBf16, dw, cols, L.width, L.width, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B))
+        return cudaErrorInvalidValue;
+    Params p{};
+    p.m = static_cast<int>(cols);
+    p.n = static_cast<int>(L.width);
+    p.num_kb = p.kb_per = static_cast<int>(ceil_div(L.rows, kBK));
+    p.n_first = 1;
+    p.inv_gain = b.inv_gain;
+    return b.dw_bn == 128 ? launch_one<128, true, kDw, kBf16, false>(ma, mb, out, p, stream)
+                          : launch_one<256, true, kDw, kBf16, false>(ma, mb, out, p, stream);
+}
+
+template <bool kBf16>
+cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
+{
+    const BackwardPlan b = plan_backward(L, L.workspace);
+    Prepare q{};
+    q.t.rows = static_cast<int>(L.rows);
+    q.t.vocab = static_cast<int>(L.vocab);
+    q.t.count = b.targets;
+    q.t.tokens = L.targets > 0 ? L.teacher_tokens : nullptr;
+    q.t.logits = L.teacher_logits;
+    q.t.logit_type = L.teacher_type;
+    q.t.inv_temperature = 1.0f / L.temperature;
+    q.t.index = b.t_index;
+    q.t.prob = b.t_prob;
+    q.labels = L.labels;
+    q.label_bytes = L.label_bytes;
+    q.ignore_index = L.ignore_index;
+    q.temperature = L.temperature;
+    q.width = static_cast<int>(L.width);
+    q.x = L.x;
+    q.x_masked = b.x_masked;
+    q.lse = L.lse_in;
+    q.grad = L.dloss;
+    q.row_lse2 = b.row_lse2;
+    q.row_gain = b.row_gain;
+    q.inv_gain = b.inv_gain;
+    const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, kPrepWarps), 4 * sm_count());
+    cudaError_t err =
+        launch_pdl(prepare_kernel, dim3(static_cast<unsigned>(blocks)), dim3(32 * kPrepWarps), stream, q);
+    if (err != cudaSuccess)
+        return err;
+    for (int64_t col0 = 0; col0 < L.vocab; col0 += b.piece) {
+        const int64_t cols = std::min(b.piece, L.vocab - col0);
+        CUtensorMap out;
+        if (!map16(&out, kBf16, b.g, L.rows, cols, b.ldg, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B))
+            return cudaErrorInvalidValue;
+        Params p{};
+        p.t_index = b.t_index;
+        p.t_prob = b.t_prob;
+        p.targets = b.targets;
+        p.row_lse2 = b.row_lse2;
+        p.row_gain = b.row_gain;
+        err = launch_logits<kGrad, kBf16>(L, b.x_masked, col0, cols, b.single, out, p, stream);
+        if (err == cudaSuccess && L.dx)
+            err = launch_dx<kBf16>(L, b, col0, cols, col0 == 0, stream);
+        if (err == cudaSuccess && L.dweight)
+            err = launch_dw<kBf16>(L, b, col0, cols, stream);
+        if (err != cudaSuccess)
+            return err;
+    }
+    if (L.dx && b.planes) {
+        const int64_t elements = L.rows * L.width;
+        const int64_t grid = std::min<int64_t>(ceil_div(elements / 8, 256), 8 * sm_count());
+        err = launch_pdl(planes_kernel<kBf16>, dim3(static_cast<unsigned>(grid)), dim3(256), stream,
+                         static_cast<const float *>(b.dx_planes), static_cast<int>(b.splits),
+                         static_cast<size_t>(elements), static_cast<const float *>(b.inv_gain),
+                         static_cast<uint4 *>(L.dx));
+    }
+    return err;
+}
+
+} // namespace
+
+int64_t vocab_loss_workspace(const VocabLossLaunch &L, bool backward)
+{
+    return backward ? plan_backward(L, nullptr).bytes : plan_forward(L, nullptr).bytes;
+}
+
+cudaError_t launch_vocab_loss(const VocabLossLaunch &L, cudaStream_t stream)
+{
+    return L.bf16 ? run_forward<true>(L, stream) : run_forward<false>(L, stream);
+}
+
+cudaError_t launch_vocab_loss_grad(const VocabLossLaunch &L, cudaStream_t stream)
+{
+    return L.bf16 ? run_backward<true>(L, stream) : run_backward<false>(L, stream);
+}
+
+int read_and_clear_token_error()
+{
+    int value = 0;
+    if (cudaMemcpyFromSymbol(&value, vocab::g_token_error, sizeof(int)) != cudaSuccess)
+        return -1;
+    const int zero = 0;
+    if (value != 0 && cudaMemcpyToSymbol(vocab::g_token_error, &zero, sizeof(int)) != cudaSuccess)
+        return -1;
+    return value;
+}
+
+cudaError_t read_and_clear_vocab_wait_error(int *site)
+{
+    int value = 0;
+    cudaError_t err = cudaMemcpyFromSymbol(&value, g_device_error, sizeof(int));
+    if (err == cudaSuccess && value != 0) {
+        const int zero = 0;
+        err = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
+    }
+    *site = value;
+    return err;
+}
+
+} // namespace lffw
