@@ -444,7 +444,8 @@ LFFW_FP8_API lffw_status lffw_layer_norm_train(const lffw_layer_norm_train_args 
  * dsum (optional) is the gradient that arrives at sum_out by the residual stream; dx is
  * then the gradient of x and of the residual alike, and may be dsum or dy itself.
  * Requirements as above; dx and/or dgamma + dbeta set; with dgamma, workspace holds
- * lffw_layer_norm_grad_workspace(rows, cols) bytes (0 for invalid arguments). */
+ * lffw_layer_norm_grad_workspace(rows, cols) bytes (0: few rows need none; -1 for
+ * invalid arguments). */
 typedef struct lffw_layer_norm_grad_args {
     size_t struct_size; /* sizeof(lffw_layer_norm_grad_args) */
     int64_t rows, cols;
@@ -486,7 +487,7 @@ LFFW_FP8_API lffw_status lffw_layer_norm_grad(const lffw_layer_norm_grad_args *a
  * G is formed piece by piece over the vocabulary and held in 16 bits (scaled by a power of
  * two so that fp16 neither overflows nor loses small probabilities); sums are fp32.
  * workspace holds lffw_vocab_loss_workspace(args, 0 for the loss, 1 for the gradients)
- * bytes (0 for invalid arguments; it depends on the shape, the targets and, for the
+ * bytes (-1 for invalid arguments; it depends on the shape, the targets and, for the
  * gradients, on whether dx is set, not on the contents).
  * Requirements: 1 <= rows <= 2^22; 1 <= vocab <= 2^22; 8 <= width <= 2^16, width % 8 == 0;
  * 16-byte aligned x, weight, dx, dweight; a workspace on a 256-byte boundary;

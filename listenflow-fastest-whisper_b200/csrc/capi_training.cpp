@@ -141,7 +141,7 @@ lffw_status lffw_layer_norm_train(const lffw_layer_norm_train_args *a, void *str
 
 int64_t lffw_layer_norm_grad_workspace(int64_t rows, int64_t cols) noexcept
 {
-    return valid_rows(rows, cols, LFFW_DT_HALF) ? lffw::layer_norm_grad_workspace(rows, cols) : 0;
+    return valid_rows(rows, cols, LFFW_DT_HALF) ? lffw::layer_norm_grad_workspace(rows, cols) : -1;
 }
 
 lffw_status lffw_layer_norm_grad(const lffw_layer_norm_grad_args *a, void *stream) noexcept
@@ -162,9 +162,11 @@ lffw_status lffw_layer_norm_grad(const lffw_layer_norm_grad_args *a, void *strea
     const lffw_status s = gate();
     if (s != LFFW_SUCCESS)
         return s;
-    if (a->dgamma != nullptr && (a->workspace == nullptr ||
-                                 a->workspace_bytes < lffw::layer_norm_grad_workspace(a->rows, a->cols)))
-        return LFFW_INVALID_ARGUMENT;
+    if (a->dgamma != nullptr) {
+        const int64_t need = lffw::layer_norm_grad_workspace(a->rows, a->cols);
+        if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))
+            return LFFW_INVALID_ARGUMENT;
+    }
     lffw::LayerNormTrainLaunch L{};
     L.rows = a->rows;
     L.cols = a->cols;
@@ -183,7 +185,7 @@ lffw_status lffw_layer_norm_grad(const lffw_layer_norm_grad_args *a, void *strea
 
 int64_t lffw_vocab_loss_workspace(const lffw_vocab_loss_args *a, int32_t grad) noexcept
 {
-    return validate_vocab(a) == LFFW_SUCCESS ? lffw::vocab_loss_workspace(vocab_launch(a), grad != 0) : 0;
+    return validate_vocab(a) == LFFW_SUCCESS ? lffw::vocab_loss_workspace(vocab_launch(a), grad != 0) : -1;
 }
 
 lffw_status lffw_vocab_loss(const lffw_vocab_loss_args *a, void *stream) noexcept

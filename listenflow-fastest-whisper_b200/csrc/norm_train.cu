@@ -41,8 +41,11 @@ struct Params {
     float *stats; // [2, rows]: mean, rstd
     const uint16_t *dy, *dsum; // backward; x holds s
     uint16_t *dx;
-    float *partial; // [blocks, 2, cols]: dgamma, dbeta
+    float *partial;         // [blocks, 2, cols] column sums of each block, or, in a cluster,
+    float *dgamma, *dbeta;  // the results themselves
 };
+
+constexpr int kClusterBlocks = 8;
 
 template <bool kBf16>
 __device__ __forceinline__ float2 unpack(uint32_t v)
@@ -198,11 +201,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Params p)
     }
 }
 
-template <int R, bool kBf16>
+// kCluster: the grid is one cluster of eight blocks, which add up their column sums through
+// distributed shared memory, so few rows need neither a workspace nor a second launch.
+template <int R, bool kBf16, bool kCluster>
 __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Params p)
 {
     __shared__ float scratch[2][kMaxGroups][16 * 2 * R];
-    extern __shared__ float column_sums[]; // [groups - 1][2][cols]
+    extern __shared__ float column_sums[]; // [groups - 1 (kCluster: groups)][2][cols]
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
     const int group = threadIdx.y, barrier = 1 + group;
@@ -275,7 +280,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Params p
             *reinterpret_cast<uint4 *>(p.dx + (row0 + i) * p.cols + col) = make_uint4(out[0], out[1], out[2], out[3]);
         }
     }
-    if (!p.partial)
+    if (!p.dgamma)
         return;
     // The block's column sums, groups in order: the result does not depend on timing.
     if (group > 0 && active) {
@@ -287,6 +292,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Params p
         }
     }
     __syncthreads();
+    float *block_sums = kCluster ? column_sums + static_cast<size_t>(p.groups - 1) * 2 * p.cols
+                                 : p.partial + static_cast<size_t>(blockIdx.x) * 2 * p.cols;
     if (group == 0 && active) {
         for (int g = 0; g + 1 < p.groups; ++g) {
             const float *other = column_sums + static_cast<size_t>(g) * 2 * p.cols + col;
@@ -296,13 +303,26 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Params p
                 dbeta[i] += other[p.cols + i];
             }
         }
-        float *out = p.partial + static_cast<size_t>(blockIdx.x) * 2 * p.cols + col;
+        float *out = block_sums + col;
 #pragma unroll
         for (int i = 0; i < 8; i += 4) {
             *reinterpret_cast<float4 *>(out + i) = make_float4(dgamma[i], dgamma[i + 1], dgamma[i + 2], dgamma[i + 3]);
             *reinterpret_cast<float4 *>(out + p.cols + i) =
                 make_float4(dbeta[i], dbeta[i + 1], dbeta[i + 2], dbeta[i + 3]);
         }
+    }
+    if (kCluster) {
+        cluster_sync();
+        const uint32_t local = smem_u32(block_sums);
+        const int thread = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
+        for (int c = blockIdx.x * threads + thread; c < 2 * p.cols; c += kClusterBlocks * threads) {
+            float v = 0.0f;
+#pragma unroll
+            for (uint32_t b = 0; b < kClusterBlocks; ++b)
+                v += ld_shared_cluster_f32(map_to_rank(local + 4u * static_cast<uint32_t>(c), b));
+            (c < p.cols ? p.dgamma : p.dbeta)[c < p.cols ? c : c - p.cols] = v;
+        }
+        cluster_sync(); // the peers' sums stay until every block has read them
     }
 }
 
@@ -355,24 +375,35 @@ bool many_rows(int64_t rows, int64_t cols, int rows_per_step)
     return rows >= static_cast<int64_t>(sm_count()) * group_count(cols) * rows_per_step;
 }
 
+// Rows that one cluster of eight blocks handles in at most four steps of its groups, as fast
+// as the whole GPU and a second launch would (20 x 1280: 4.2 + 2.1 us and the launch against
+// one of 5 us).
+bool one_cluster(int64_t rows, int64_t cols)
+{
+    return rows <= 4 * int64_t{kClusterBlocks} * group_count(cols) * kBackwardRows;
+}
+
 int backward_blocks(int64_t rows, int64_t cols)
 {
     return grid_blocks(rows, cols, many_rows(rows, cols, kBackwardRows) ? kBackwardRows : 1);
 }
 
 template <class Kernel>
-cudaError_t launch_groups(Kernel kernel, int blocks, int64_t cols, size_t smem, cudaStream_t stream, const Params &p)
+cudaError_t launch_groups(Kernel kernel, int blocks, int cluster, size_t smem, cudaStream_t stream, const Params &p)
 {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(blocks));
-    config.blockDim = dim3(static_cast<unsigned>(group_threads(cols)), static_cast<unsigned>(group_count(cols)));
+    config.blockDim = dim3(static_cast<unsigned>(p.group_threads), static_cast<unsigned>(p.groups));
     config.dynamicSmemBytes = smem;
     config.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = attr;
-    config.numAttrs = 1;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+    config.attrs = attrs;
+    config.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t err = cudaLaunchKernelEx(&config, kernel, p);
     count_launch();
     return err != cudaSuccess ? err : cudaGetLastError();
@@ -382,26 +413,37 @@ template <bool kBf16>
 cudaError_t run_forward(const LayerNormTrainLaunch &L, const Params &p, cudaStream_t stream)
 {
     if (many_rows(L.rows, L.cols, kForwardRows))
-        return launch_groups(forward_kernel<kForwardRows, kBf16>, grid_blocks(L.rows, L.cols, kForwardRows), L.cols, 0,
+        return launch_groups(forward_kernel<kForwardRows, kBf16>, grid_blocks(L.rows, L.cols, kForwardRows), 1, 0,
                              stream, p);
-    return launch_groups(forward_kernel<1, kBf16>, grid_blocks(L.rows, L.cols, 1), L.cols, 0, stream, p);
+    return launch_groups(forward_kernel<1, kBf16>, grid_blocks(L.rows, L.cols, 1), 1, 0, stream, p);
 }
 
+// Shared memory of the column sums: groups x 2 x cols floats, where groups x cols is at most
+// 640 threads' 8 columns each (40 KB), under the 48 KB that every launch may use.
 template <bool kBf16>
 cudaError_t run_backward(const LayerNormTrainLaunch &L, const Params &p, cudaStream_t stream)
 {
-    // At most (14 groups - 1) x 2 x 256 columns or the like: under the 48 KB every launch may use.
-    const size_t smem = p.partial ? static_cast<size_t>(p.groups - 1) * 2 * L.cols * sizeof(float) : 0;
+    const size_t sums = L.dgamma ? 2 * L.cols * sizeof(float) : 0;
+    if (L.dgamma && one_cluster(L.rows, L.cols))
+        return launch_groups(backward_kernel<kBackwardRows, kBf16, true>, kClusterBlocks, kClusterBlocks,
+                             p.groups * sums, stream, p);
     const int blocks = backward_blocks(L.rows, L.cols);
-    return many_rows(L.rows, L.cols, kBackwardRows)
-               ? launch_groups(backward_kernel<kBackwardRows, kBf16>, blocks, L.cols, smem, stream, p)
-               : launch_groups(backward_kernel<1, kBf16>, blocks, L.cols, smem, stream, p);
+    cudaError_t err = many_rows(L.rows, L.cols, kBackwardRows)
+                          ? launch_groups(backward_kernel<kBackwardRows, kBf16, false>, blocks, 1,
+                                          (p.groups - 1) * sums, stream, p)
+                          : launch_groups(backward_kernel<1, kBf16, false>, blocks, 1, (p.groups - 1) * sums, stream, p);
+    if (err == cudaSuccess && L.dgamma)
+        err = launch_pdl(columns_kernel, dim3(static_cast<unsigned>((2 * L.cols + 31) / 32)), dim3(1024), stream,
+                         static_cast<const float *>(p.partial), blocks, p.cols, L.dgamma, L.dbeta);
+    return err;
 }
 
 } // namespace
 
 int64_t layer_norm_grad_workspace(int64_t rows, int64_t cols)
 {
+    if (one_cluster(rows, cols))
+        return 0;
     return static_cast<int64_t>(backward_blocks(rows, cols)) * 2 * cols * static_cast<int64_t>(sizeof(float));
 }
 
@@ -436,12 +478,10 @@ cudaError_t launch_layer_norm_backward(const LayerNormTrainLaunch &L, cudaStream
     p.dx = L.dx;
     p.gamma = L.gamma;
     p.stats = L.stats;
-    p.partial = L.dgamma ? static_cast<float *>(L.workspace) : nullptr;
-    const cudaError_t err = L.bf16 ? run_backward<true>(L, p, stream) : run_backward<false>(L, p, stream);
-    if (err != cudaSuccess || !L.dgamma)
-        return err;
-    return launch_pdl(columns_kernel, dim3(static_cast<unsigned>((2 * L.cols + 31) / 32)), dim3(1024), stream,
-                      static_cast<const float *>(p.partial), backward_blocks(L.rows, L.cols), p.cols, L.dgamma, L.dbeta);
+    p.partial = static_cast<float *>(L.workspace);
+    p.dgamma = L.dgamma;
+    p.dbeta = L.dbeta;
+    return L.bf16 ? run_backward<true>(L, p, stream) : run_backward<false>(L, p, stream);
 }
 
 } // namespace lffw

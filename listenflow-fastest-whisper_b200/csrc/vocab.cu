@@ -28,6 +28,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "host_util.cuh"
 #include "launch.h"
@@ -40,9 +41,10 @@ namespace vocab {
 constexpr int kBM = 128;               // accumulator rows per CTA (TMEM lanes)
 constexpr int kBK = 64;                // K elements per stage: one 128-byte swizzle row
 constexpr int kUmmaK = 16;             // K of one kind::f16 MMA
-constexpr int kEpiWarps = 8;           // two per TMEM lane quarter, each with half of the tile's columns
-constexpr int kThreads = 64 + 32 * kEpiWarps; // warp 0 TMA, warp 1 MMA, warps 2-9 epilogue
+constexpr int kEpiWarps = 16;          // four per TMEM lane quarter, each with a quarter of the tile's columns
+constexpr int kThreads = 64 + 32 * kEpiWarps; // warp 0 TMA, warp 1 MMA, warps 2-17 epilogue
 constexpr int kSub = 32;               // columns per epilogue step
+constexpr int kMaxBN = 256;            // widest tile
 constexpr float kLog2e = 1.4426950408889634f;
 
 enum Mode : int { kStats, kGrad, kDx, kDw };
@@ -50,25 +52,28 @@ enum Mode : int { kStats, kGrad, kDx, kDw };
 // A label or a teacher token outside the vocabulary was met (see lffw_vocab_loss_error).
 __device__ int g_token_error = 0;
 
-// kPair: a cluster of two CTAs computes a 256 x BN tile with cta_group::2 MMAs, each CTA
-// holding 128 rows of A, BN/2 rows of B and its half of the accumulator: per SM that halves
-// the B traffic, which a 128 x 256 tile of one CTA would need at 96 B/clk, above what the
-// L2 delivers.
+// kPair: a cluster of two CTAs computes a 256 x bn tile with cta_group::2 MMAs, each CTA
+// holding 128 rows of A, bn/2 rows of B and its half of the accumulator.  At 256 x 256 an SM's
+// shared memory then takes 64 B/clk of TMA writes and 64 B/clk of MMA reads, its 128 B/clk; a
+// 128 x 256 tile of one CTA would want 192.
 // Operand layouts in shared memory (128-byte swizzle either way):
 //   K-major   rows of 64 K elements, one TMA box
 //   MN-major  64 K rows of 64 MN elements per TMA box, boxes stacked along MN
 // x and W are K-major for z = x W^T; W is MN-major as B of G W; G and x are MN-major in G^T x.
-template <int BN, bool kPair, int MODE>
+// The tile width bn (a multiple of 16, of 32 in a pair, up to 256) is a launch parameter: the last dimension is
+// cut into equal tiles instead of 256-wide ones and a remainder, and small problems into as
+// many as the SMs share evenly.
+template <bool kPair, int MODE>
 struct Cfg {
     static constexpr bool kAMn = MODE == kDw;
     static constexpr bool kBMn = MODE == kDx || MODE == kDw;
     static constexpr int kTileM = kPair ? 2 * kBM : kBM;
-    static constexpr int kBRows = kPair ? BN / 2 : BN; // B rows this CTA loads
     static constexpr int kABytes = kBM * 128;
-    static constexpr int kBBytes = kBRows * 128;
+    static constexpr int kBBytes = (kPair ? kMaxBN / 2 : kMaxBN) * 128; // this CTA's rows of B, at most
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kTxBytes = kPair ? 2 * kStageBytes : kStageBytes;
-    static constexpr int kStaging = MODE == kStats ? 0 : 4096; // per epilogue warp
+    // Per epilogue warp: kStats exchanges (maximum, sum, target product) of 32 rows, twice
+    // (tile parity); the others stage a 32-row x 64-byte store.
+    static constexpr int kStaging = MODE == kStats ? 2 * 3 * 32 * 4 : 2048;
     static constexpr int kBarBytes = 256;
     static constexpr int kBudget = 232448 - 1024;
     static constexpr int kFit = (kBudget - kEpiWarps * kStaging - kBarBytes) / kStageBytes;
@@ -77,12 +82,10 @@ struct Cfg {
     static constexpr int kOffStaging = kOffB + kStages * kBBytes;
     static constexpr int kOffBar = kOffStaging + kEpiWarps * kStaging;
     static constexpr int kSmemBytes = kOffBar + kBarBytes + 1024;
-    static constexpr int kTmemCols = 2 * BN; // two accumulators
-    static constexpr int kSlice = BN / 2;    // columns per epilogue warp
+    static constexpr int kTmemCols = 2 * kMaxBN; // two accumulators
+    // Instruction descriptor without its operand types and N.
     static constexpr uint32_t kIdesc = (1u << 4) | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u) |
-                                       (static_cast<uint32_t>(BN >> 3) << 17) |
                                        (static_cast<uint32_t>(kTileM >> 4) << 24);
-    static_assert(BN == 128 || BN == 256, "tile width");
     static_assert(kStages >= 4 && kSmemBytes <= 232448, "shared memory budget");
     static_assert((2 * kStages + 5) * 8 + 8 <= kBarBytes, "barrier area");
 };
@@ -90,9 +93,11 @@ struct Cfg {
 struct Params {
     int m, n;                    // rows and columns of the output
     int m_tiles, n_tiles, num_tiles;
+    int bn;                      // tile width
+    int a_rows;                  // rows of a K-major A tile that are loaded (kBM, or few rows rounded up)
     int num_kb, kb_per;          // K blocks, and how many of them one split sums
     int n_first;                 // raster: 0 = M tiles fastest, 1 = N tiles fastest
-    uint32_t type_bits;          // instruction descriptor's operand types
+    uint32_t idesc_bits;         // instruction descriptor's operand types and N
     // kStats and kGrad: row i is token i, column c is vocabulary entry col0 + c.
     int col0;
     float scale2;                // log2(e) / T
@@ -114,6 +119,14 @@ __device__ __forceinline__ float exp2_approx(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Hands a drained accumulator back to the MMA issuer.  The reads of it have completed
+// (tcgen05.wait::ld), so the arrival orders nothing else: a release at cluster scope would
+// wait for this warp's global stores as well (it was a sixth of the epilogue's stalls).
+__device__ __forceinline__ void release_accumulator(uint32_t cluster_bar)
+{
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16)
@@ -212,12 +225,12 @@ __device__ __forceinline__ uint64_t desc_mn_boxes(uint32_t addr)
 
 // tm_a, tm_b: operands.  tm_out: G (kGrad), dW (kDw), dx itself or the fp32 planes (kDx).
 // Planes is the kDx form that writes fp32 planes instead of dx.
-template <int BN, bool kPair, int MODE, bool kBf16, bool kPlanes>
+template <bool kPair, int MODE, bool kBf16, bool kPlanes>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                 const __grid_constant__ CUtensorMap tm_out, const Params p)
 {
-    using C = Cfg<BN, kPair, MODE>;
+    using C = Cfg<kPair, MODE>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     uint8_t *smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
@@ -249,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int nt = p.n_first ? r % p.n_tiles : r / p.m_tiles;
         Tile tile;
         tile.m0 = mt * C::kTileM + static_cast<int>(rank) * kBM;
-        tile.n0 = nt * BN;
+        tile.n0 = nt * p.bn;
         tile.split = split;
         tile.kb0 = split * p.kb_per;
         tile.kbn = min(p.kb_per, p.num_kb - tile.kb0);
@@ -307,9 +320,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 else
                     tma_load_2d(dst, map, full, x, y);
             };
+            const int b_rows = kPair ? p.bn / 2 : p.bn; // this CTA's
+            const int b_boxes = (b_rows + 63) / 64;     // MN-major
+            const uint32_t tx = (kPair ? 2u : 1u) * (static_cast<uint32_t>(C::kAMn ? kBM : p.a_rows) * 128u +
+                                                     (C::kBMn ? b_boxes * 8192u : b_rows * 128u));
             for (int t = tile_first; ok && t < p.num_tiles; t += tile_step) {
                 const Tile tile = tile_at(t);
-                const int b0 = tile.n0 + static_cast<int>(rank) * C::kBRows;
+                const int b0 = tile.n0 + static_cast<int>(rank) * b_rows;
                 for (int i = 0; i < tile.kbn; ++i) {
                     if (!mbar_wait(bar_empty + 8 * s, ph ^ 1u, kSiteProducerEmpty)) {
                         ok = false;
@@ -317,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     const int k0 = (tile.kb0 + i) * kBK;
                     if (leader)
-                        mbar_arrive_expect_tx(bar_full + 8 * s, C::kTxBytes);
+                        mbar_arrive_expect_tx(bar_full + 8 * s, tx);
                     const uint32_t full = kPair ? map_to_rank(bar_full + 8 * s, 0) : bar_full + 8 * s;
                     const uint32_t a = sbase + s * C::kABytes;
                     const uint32_t b = sbase + C::kOffB + s * C::kBBytes;
@@ -329,8 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         load(a, &tm_a, full, k0, tile.m0);
                     }
                     if (C::kBMn) {
-#pragma unroll
-                        for (int j = 0; j < C::kBRows / 64; ++j)
+                        for (int j = 0; j < b_boxes; ++j)
                             load(b + j * 8192, &tm_b, full, b0 + 64 * j, k0);
                     } else {
                         load(b, &tm_b, full, k0, b0);
@@ -356,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
         // ---------------- MMA issuer (one thread of the leader) ----------------
         if (lane == 0 && leader) {
-            const uint32_t idesc = C::kIdesc | p.type_bits;
+            const uint32_t idesc = C::kIdesc | p.idesc_bits;
             int s = 0;
             uint32_t ph = 0;
             int local = 0;
@@ -373,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     break;
                 }
                 tc_fence_after();
-                const uint32_t d_tmem = tmem_base + a * BN;
+                const uint32_t d_tmem = tmem_base + a * kMaxBN;
                 for (int i = 0; i < tile.kbn; ++i) {
                     if (!mbar_wait(bar_full + 8 * s, ph, kSiteMmaFull)) {
                         ok = false;
@@ -419,15 +435,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else {
-        // ---------------- Epilogue: 8 independent warps, one row per lane ----------------
+        // ---------------- Epilogue: 16 warps, one row per lane ----------------
         const int ew = warp - 2;
         const int quarter = warp & 3;
-        const int half = ew >> 2; // this warp's half of the tile's columns
+        // This warp's columns: of the tile's 32-column steps, about a quarter.
+        const int slice = ew >> 2;
+        const int steps = (p.bn + kSub - 1) / kSub;
+        const int col_begin = slice * steps / 4 * kSub;
+        const int col_end = min((slice + 1) * steps / 4 * kSub, p.bn);
         const uint32_t acc_empty = kPair ? map_to_rank(bar_acc_empty, 0) : bar_acc_empty;
         uint8_t *staging = smem + C::kOffStaging + ew * C::kStaging;
         const uint32_t staging_s = smem_u32(staging);
         const float inv_gain = MODE == kDw || (MODE == kDx && !kPlanes) ? *p.inv_gain : 1.0f;
-        int local = 0, stores = 0;
+        int local = 0;
         for (int t = tile_first; t < p.num_tiles; t += tile_step) {
             const Tile tile = tile_at(t);
             if (tile.kbn <= 0)
@@ -437,10 +457,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++local;
             const int row0 = tile.m0 + quarter * 32;
             const int row = row0 + lane;
-            const int col0 = tile.n0 + half * C::kSlice;
+            const int col0 = tile.n0 + col_begin;
+            const int col1 = min(tile.n0 + col_end, p.n);
             // Rows and columns of this warp that exist.
-            const int width = row0 < p.m ? min(C::kSlice, p.n - col0) : 0;
-            const int subs = width > 0 ? (width + kSub - 1) / kSub : 0;
+            const int width = row0 < p.m ? col1 - col0 : 0;
+            int subs = width > 0 ? (width + kSub - 1) / kSub : 0;
 
             // The row's next target column (relative to the piece), found while the MMAs run.
             int next = INT_MAX, entry = 0;
@@ -465,10 +486,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             float run_max = -INFINITY, run_sum = 0.0f, run_t = 0.0f;
 
             const bool ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_full + 8 * a, acc_ph, kSiteEpilogueAccFull));
-            if (!ok)
-                break;
+            if (!ok) {
+                if (MODE != kStats)
+                    break;
+                subs = 0; // the error word is set; keep meeting the quarter's other warps
+            }
             tc_fence_after();
-            const uint32_t t_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + a * BN + half * C::kSlice;
+            const uint32_t t_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + a * kMaxBN + col_begin;
 #pragma unroll 1
             for (int sub = 0; sub < subs; ++sub) {
                 const int c0 = col0 + sub * kSub;
@@ -480,18 +504,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                     if (lane == 0) {
                         if (kPair)
-                            mbar_arrive_cluster(acc_empty + 8 * a);
+                            release_accumulator(acc_empty + 8 * a);
                         else
                             mbar_arrive(acc_empty + 8 * a);
                     }
                 }
                 if (MODE == kStats) {
                     // Running maximum and sum of exp2(scale2 z - maximum).
-                    if (p.n - c0 < kSub) {
+                    if (col1 - c0 < kSub) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (c0 + i >= p.n)
-                                v[i] = 0xff800000u; // columns past the vocabulary: -infinity
+                            if (c0 + i >= col1)
+                                v[i] = 0xff800000u; // columns past the tile or the vocabulary: -infinity
                     }
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -514,8 +538,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     run_sum = fmaf(run_sum, exp2_approx(run_max - next_max), acc[0].x + acc[0].y);
                     run_max = next_max;
                     // Targets of this step: rare, so one uniform test in the common case.
-                    while (__any_sync(0xffffffffu, next < c0 + kSub)) {
-                        if (next < c0 + kSub) {
+                    const int step_end = min(c0 + kSub, col1);
+                    while (__any_sync(0xffffffffu, next < step_end)) {
+                        if (next < step_end) {
                             const float z = select32(v, next - c0);
                             if (p.t_index) {
                                 run_t = fmaf(p.t_prob[static_cast<size_t>(row) * p.targets + entry], z, run_t);
@@ -529,7 +554,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     continue;
                 }
-                uint32_t h[16];
                 float f[32];
                 if (MODE == kGrad) {
                     const float2 ref = make_float2(-lse2, -lse2);
@@ -557,43 +581,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int i = 0; i < 32; ++i)
                         f[i] = __uint_as_float(v[i]) * inv_gain;
                 }
-                if (MODE == kDx && kPlanes) {
-                    // 32 rows x 128 B of fp32, 128-byte swizzle: chunk j of row r at j ^ (r & 7).
+                // Staging: 32 rows x 64 B, 64-byte swizzle: chunk j of row r at j ^ ((r >> 1) & 3).
+                constexpr int kSteps = MODE == kDx && kPlanes ? 2 : 1; // fp32: 16 columns at a time
+#pragma unroll
+                for (int hf = 0; hf < kSteps; ++hf) {
                     if (lane == 0)
-                        bulk_wait_group_read0();
+                        bulk_wait_group_read0(); // the previous store has read the buffer
                     __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        *reinterpret_cast<float4 *>(staging + lane * 128 + ((j ^ (lane & 7)) * 16)) =
-                            make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (p.accumulate)
-                            tma_store_add_3d(&tm_out, staging_s, c0, row0, tile.split);
-                        else
-                            tma_store_3d(&tm_out, staging_s, c0, row0, tile.split);
-                        bulk_commit_group();
+                    for (int j = 0; j < 4; ++j) {
+                        uint4 w;
+                        if (kSteps == 2) {
+                            w = make_uint4(__float_as_uint(f[16 * hf + 4 * j]), __float_as_uint(f[16 * hf + 4 * j + 1]),
+                                           __float_as_uint(f[16 * hf + 4 * j + 2]),
+                                           __float_as_uint(f[16 * hf + 4 * j + 3]));
+                        } else {
+                            w = make_uint4(pack16(f[8 * j], f[8 * j + 1], kBf16), pack16(f[8 * j + 2], f[8 * j + 3], kBf16),
+                                           pack16(f[8 * j + 4], f[8 * j + 5], kBf16),
+                                           pack16(f[8 * j + 6], f[8 * j + 7], kBf16));
+                        }
+                        *reinterpret_cast<uint4 *>(staging + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) = w;
                     }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        h[i] = pack16(f[2 * i], f[2 * i + 1], kBf16);
-                    // Two buffers of 32 rows x 64 B, 64-byte swizzle: chunk j of row r at
-                    // j ^ ((r >> 1) & 3).  All but the newest store have read theirs.
-                    const uint32_t buf = (stores & 1) * 2048u;
-                    ++stores;
-                    if (lane == 0)
-                        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                    __syncwarp();
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        *reinterpret_cast<uint4 *>(staging + buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) =
-                            make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        tma_store_2d(&tm_out, staging_s + buf, c0, row0);
+                        if (kSteps == 2) {
+                            if (c0 + 16 * hf < p.n) {
+                                if (p.accumulate)
+                                    tma_store_add_3d(&tm_out, staging_s, c0 + 16 * hf, row0, tile.split);
+                                else
+                                    tma_store_3d(&tm_out, staging_s, c0 + 16 * hf, row0, tile.split);
+                            }
+                        } else {
+                            tma_store_2d(&tm_out, staging_s, c0, row0);
+                        }
                         bulk_commit_group();
                     }
                 }
@@ -603,17 +624,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) {
                     if (kPair)
-                        mbar_arrive_cluster(acc_empty + 8 * a);
+                        release_accumulator(acc_empty + 8 * a);
                     else
                         mbar_arrive(acc_empty + 8 * a);
                 }
             }
-            if (MODE == kStats && subs > 0 && row < p.m) {
-                const size_t at = static_cast<size_t>(col0 / C::kSlice) * p.m + row;
-                p.part_max[at] = run_max;
-                p.part_sum[at] = run_sum;
-                if (p.part_t)
-                    p.part_t[at] = run_t;
+            if (MODE == kStats) {
+                // Merge the four column slices of each row: the warps of a quarter meet on a
+                // named barrier, and the first writes the tile's partial result.
+                float *mine = reinterpret_cast<float *>(staging) + (local & 1) * 96;
+                mine[lane] = run_max;
+                mine[32 + lane] = run_sum;
+                mine[64 + lane] = run_t;
+                named_barrier_sync(1 + quarter, 128);
+                if (slice == 0 && row < p.m) {
+#pragma unroll
+                    for (int j = 1; j < 4; ++j) {
+                        const float *other = mine + j * (4 * C::kStaging / 4);
+                        const float m = other[lane];
+                        const float next_max = fmaxf(run_max, m);
+                        run_sum = fmaf(run_sum, exp2_approx(run_max - next_max),
+                                       other[32 + lane] * (m == -INFINITY ? 0.0f : exp2_approx(m - next_max)));
+                        run_max = next_max;
+                        run_t += other[64 + lane];
+                    }
+                    const size_t at = static_cast<size_t>(tile.n0 / p.bn) * p.m + row;
+                    p.part_max[at] = run_max;
+                    p.part_sum[at] = run_sum;
+                    if (p.part_t)
+                        p.part_t[at] = run_t;
+                }
             }
         }
         if (MODE != kStats && lane == 0)
@@ -645,7 +685,6 @@ __device__ __forceinline__ float load_float(const void *p, int dtype, size_t i)
 }
 
 constexpr int kPrepWarps = 8;
-constexpr int kPerLane = kVocabMaxTargets / 32;
 
 struct Targets {
     int rows, vocab, count;
@@ -657,71 +696,91 @@ struct Targets {
     float *prob;
 };
 
-// One warp lays out one row's teacher entries: the softmax of the logits of the valid ones
-// (token in the vocabulary, logit not -infinity) and their columns in ascending order, by
-// ranks (stable, so equal tokens keep their order), the rest INT_MAX.  Returns whether the
-// row has any, with (negative entropy, sum) of its probabilities in 64 bits: the loss is a
-// difference of terms near log(V), so it is formed from unrounded ones.
-__device__ __forceinline__ bool sort_targets(const Targets &t, int row, int lane, int32_t *cols, double &entropy,
+// Ascending bitonic sort of 32 R keys over a warp: key i of lane l is element 32 i + l, so
+// distances from 32 up stay in a lane's registers and the others are lane exchanges.
+template <int R>
+__device__ __forceinline__ void sort_keys(uint32_t (&key)[R], int lane)
+{
+#pragma unroll
+    for (int size = 2; size <= 32 * R; size *= 2) {
+#pragma unroll
+        for (int dist = size / 2; dist > 0; dist /= 2) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int e = 32 * i + lane;
+                if (dist >= 32) {
+                    const int j = i ^ (dist / 32);
+                    if (j > i) {
+                        const uint32_t lo = min(key[i], key[j]), hi = max(key[i], key[j]);
+                        const bool up = (e & size) == 0;
+                        key[i] = up ? lo : hi;
+                        key[j] = up ? hi : lo;
+                    }
+                } else {
+                    const uint32_t other = __shfl_xor_sync(0xffffffffu, key[i], dist);
+                    const bool up = (e & size) == 0, low = (lane & dist) == 0;
+                    key[i] = up == low ? min(key[i], other) : max(key[i], other);
+                }
+            }
+        }
+    }
+}
+
+// One warp lays out one row's teacher entries (up to 32 R): the softmax of the logits of the
+// valid ones (token in the vocabulary, logit not -infinity) and their columns in ascending
+// order, the rest INT_MAX.  A sort key is the column with the entry's number below it (22 + 8
+// bits), so equal tokens keep their order.  Returns whether the row has any, with (negative
+// entropy, sum) of its probabilities in 64 bits: the loss is a difference of terms near
+// log(V), so it is formed from unrounded ones.
+template <int R>
+__device__ __forceinline__ bool sort_targets(const Targets &t, int row, int lane, float *probs, double &entropy,
                                              double &total)
 {
+    constexpr uint32_t kNone = 0xFFFFFFFFu;
     const size_t base = static_cast<size_t>(row) * t.count;
-    int32_t col[kPerLane];
-    float z[kPerLane];
-    float top = -INFINITY;
+    int32_t token[R];
+    float z[R];
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
+    for (int i = 0; i < R; ++i) {
         const int j = lane + 32 * i;
-        col[i] = INT_MAX;
-        z[i] = -INFINITY;
-        if (j < t.count) {
-            const int32_t token = t.tokens[base + j];
-            if (token >= t.vocab)
-                g_token_error = 1;
-            if (token >= 0 && token < t.vocab) {
-                z[i] = load_float(t.logits, t.logit_type, base + j) * t.inv_temperature;
-                col[i] = z[i] == -INFINITY ? INT_MAX : token;
-            }
-            cols[j] = col[i];
-        }
+        token[i] = j < t.count ? t.tokens[base + j] : -1;
+        z[i] = j < t.count ? load_float(t.logits, t.logit_type, base + j) * t.inv_temperature : 0.0f;
+    }
+    uint32_t key[R];
+    float top = -INFINITY;
+    bool has = false;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (token[i] >= t.vocab)
+            g_token_error = 1;
+        const bool valid = token[i] >= 0 && token[i] < t.vocab && z[i] != -INFINITY;
+        key[i] = valid ? (static_cast<uint32_t>(token[i]) << 8) | static_cast<uint32_t>(lane + 32 * i) : kNone;
+        z[i] = valid ? z[i] : -INFINITY;
+        has |= valid;
         top = fmaxf(top, z[i]);
     }
+    const bool any = __any_sync(0xffffffffu, has);
 #pragma unroll
     for (int o = 16; o; o >>= 1)
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float e[kPerLane], sum = 0.0f;
+    float e[R], sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-        e[i] = col[i] == INT_MAX ? 0.0f : exp2f((z[i] - top) * kLog2e);
+    for (int i = 0; i < R; ++i) {
+        e[i] = key[i] == kNone ? 0.0f : exp2f((z[i] - top) * kLog2e);
         sum += e[i];
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1)
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    __syncwarp();
-    const bool any = __any_sync(0xffffffffu, [&] {
-        bool has = false;
-#pragma unroll
-        for (int i = 0; i < kPerLane; ++i)
-            has |= col[i] != INT_MAX;
-        return has;
-    }());
     entropy = 0.0;
     total = 0.0;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-        const int j = lane + 32 * i;
-        if (j < t.count) {
-            int rank = 0;
-            for (int o = 0; o < t.count; ++o)
-                rank += cols[o] < col[i] || (cols[o] == col[i] && o < j);
-            const float prob = any ? e[i] / sum : 0.0f;
-            t.index[base + rank] = col[i];
-            t.prob[base + rank] = prob;
-            if (col[i] != INT_MAX) {
-                entropy += static_cast<double>(prob) * (static_cast<double>(z[i]) - static_cast<double>(top));
-                total += prob;
-            }
+    for (int i = 0; i < R; ++i) {
+        const float prob = any ? e[i] / sum : 0.0f;
+        probs[lane + 32 * i] = prob;
+        if (key[i] != kNone) {
+            entropy += static_cast<double>(prob) * (static_cast<double>(z[i]) - static_cast<double>(top));
+            total += prob;
         }
     }
 #pragma unroll
@@ -731,20 +790,31 @@ __device__ __forceinline__ bool sort_targets(const Targets &t, int row, int lane
     }
     if (any)
         entropy -= total * log(static_cast<double>(sum));
+    sort_keys<R>(key, lane);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int j = lane + 32 * i;
+        if (j < t.count) {
+            t.index[base + j] = key[i] == kNone ? INT_MAX : static_cast<int32_t>(key[i] >> 8);
+            t.prob[base + j] = key[i] == kNone ? 0.0f : probs[key[i] & 255u];
+        }
+    }
     __syncwarp();
     return any;
 }
 
 // Forward of the distillation: sorted targets, and (entropy, sum) per row.
+template <int R>
 __global__ void __launch_bounds__(32 * kPrepWarps) targets_kernel(const Targets t, double2 *row_terms)
 {
-    __shared__ int32_t cols[kPrepWarps][kVocabMaxTargets];
+    __shared__ float probs[kPrepWarps][32 * R];
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     for (int row = blockIdx.x * kPrepWarps + warp; row < t.rows; row += gridDim.x * kPrepWarps) {
         double entropy, total;
-        sort_targets(t, row, lane, cols[warp], entropy, total);
+        sort_targets<R>(t, row, lane, probs[warp], entropy, total);
         if (lane == 0)
             row_terms[row] = make_double2(entropy, total);
     }
@@ -767,17 +837,20 @@ struct Prepare {
 // without a target are zero, so that whatever those hold (NaN included) reaches neither G nor
 // dW.  s = 2^(13 - exponent of max |g T|) puts |g T s| in [2^13, 2^14): with |p - t| <= 1, G
 // then fits fp16 and keeps 11 bits down to p = 2^-28.
+// R = 0: one label per row; otherwise up to 32 R teacher entries.
+template <int R>
 __global__ void __launch_bounds__(32 * kPrepWarps) prepare_kernel(const Prepare p)
 {
-    __shared__ int32_t cols[kPrepWarps][kVocabMaxTargets];
+    __shared__ float probs[kPrepWarps][R > 0 ? 32 * R : 1];
     __shared__ float warp_max[kPrepWarps];
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     // The largest finite |g|: every block reads all of them (a few KB).
     float top = 0.0f;
-    for (int i = threadIdx.x; i < p.t.rows; i += blockDim.x) {
-        const float g = fabsf(p.grad[i]);
+#pragma unroll 8
+    for (int i = threadIdx.x; i < p.t.rows; i += 32 * kPrepWarps) {
+        const float g = fabsf(__ldg(p.grad + i));
         top = fmaxf(top, g < INFINITY ? g : 0.0f);
     }
 #pragma unroll
@@ -797,10 +870,20 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_kernel(const Prepare 
         *p.inv_gain = ldexpf(1.0f, exponent - 13);
 
     for (int row = blockIdx.x * kPrepWarps + warp; row < p.t.rows; row += gridDim.x * kPrepWarps) {
+        const int vectors = p.width / 8;
+        const size_t base = static_cast<size_t>(row) * vectors;
+        const uint4 *src = static_cast<const uint4 *>(p.x) + base;
+        uint4 *dst = static_cast<uint4 *>(p.x_masked) + base;
+        // The row's first 1280 elements are requested before its targets are known.
+        uint4 head[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+            if (lane + 32 * i < vectors)
+                head[i] = __ldg(src + lane + 32 * i);
         bool any;
-        if (p.t.tokens) {
+        if constexpr (R > 0) {
             double entropy, total;
-            any = sort_targets(p.t, row, lane, cols[warp], entropy, total);
+            any = sort_targets<R>(p.t, row, lane, probs[warp], entropy, total);
         } else {
             const int64_t label = load_label(p.labels, p.label_bytes, row);
             any = label != p.ignore_index && label >= 0 && label < p.t.vocab;
@@ -815,21 +898,23 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_kernel(const Prepare 
             p.row_lse2[row] = any ? p.lse[row] * kLog2e : 0.0f;
             p.row_gain[row] = any ? p.grad[row] * p.temperature * s : 0.0f;
         }
-        const size_t base = static_cast<size_t>(row) * (p.width / 8);
-        const uint4 *src = static_cast<const uint4 *>(p.x) + base;
-        uint4 *dst = static_cast<uint4 *>(p.x_masked) + base;
-        for (int i = lane; i < p.width / 8; i += 32)
-            dst[i] = any ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+            if (lane + 32 * i < vectors)
+                dst[lane + 32 * i] = any ? head[i] : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = lane + 160; i < vectors; i += 32)
+            dst[i] = any ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
 // ---- forward's last step ---------------------------------------------------------
 
 struct Combine {
-    int rows, slices, vocab;
+    int rows, slices, vocab, width;
     const float *part_max, *part_sum, *part_t;
     const float *label_z;
-    const void *labels;
+    const void *x, *weight;
+    const void *labels; // one per row, or null with the teacher's row_terms
     int label_bytes;
     int64_t ignore_index;
     const double2 *row_terms;
@@ -837,48 +922,56 @@ struct Combine {
     float *losses, *lse;
 };
 
-constexpr int kCombineGroups = 32;
-
-// Merges the slices' maxima and sums (and target products) of 32 rows per block, lane = row,
-// in a fixed order; the loss is formed in 64 bits because it is a difference of terms near
-// log(V).
-__global__ void __launch_bounds__(32 * kCombineGroups) combine_kernel(const Combine p)
+template <bool kBf16>
+__device__ __forceinline__ float dot16(uint4 a, uint4 b, float acc)
 {
-    __shared__ float s_max[kCombineGroups][32], s_sum[kCombineGroups][32];
-    __shared__ double s_t[kCombineGroups][32];
-    griddepcontrol_wait();
-    griddepcontrol_launch_dependents();
-    const int group = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int row = blockIdx.x * 32 + lane;
-    float mx = -INFINITY, sum = 0.0f;
-    double target = 0.0;
-    if (row < p.rows) {
-#pragma unroll 4
-        for (int i = group; i < p.slices; i += kCombineGroups) {
-            const size_t at = static_cast<size_t>(i) * p.rows + row;
-            const float m = p.part_max[at], s = p.part_sum[at];
-            if (p.part_t)
-                target += p.part_t[at];
-            const float next = fmaxf(mx, m);
-            sum = fmaf(sum, exp2f(mx - next), s * exp2f(m - next));
-            mx = next;
+    const uint32_t *u = &a.x, *v = &b.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float2 p, q;
+        if (kBf16) {
+            p = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xFFFF0000u));
+            q = make_float2(__uint_as_float(v[i] << 16), __uint_as_float(v[i] & 0xFFFF0000u));
+        } else {
+            __half2 h, k;
+            memcpy(&h, &u[i], 4);
+            memcpy(&k, &v[i], 4);
+            p = __half22float2(h);
+            q = __half22float2(k);
         }
+        acc = fmaf(p.x, q.x, acc);
+        acc = fmaf(p.y, q.y, acc);
     }
-    s_max[group][lane] = mx;
-    s_sum[group][lane] = sum;
-    s_t[group][lane] = target;
-    __syncthreads();
-    if (group != 0 || row >= p.rows)
-        return;
-    for (int i = 1; i < kCombineGroups && i < p.slices; ++i) {
-        const float m = s_max[i][lane];
-        const float next = fmaxf(mx, m);
-        sum = fmaf(sum, exp2f(mx - next), s_sum[i][lane] * exp2f(m - next));
-        mx = next;
-        target += s_t[i][lane];
+    return acc;
+}
+
+// The label's logit as an fp32 dot product by one warp (0 for a label outside the vocabulary).
+// The tensor cores truncate each of the width / 16 steps of a logit's sum, which shifts large
+// logits, the label's above all, by some 1e-6 of their value.  One dot product per row
+// replaces the label's logit where it enters: the loss and, by its probability, the lse.
+template <bool kBf16>
+__device__ __forceinline__ float label_product(const Combine &p, int row, int lane)
+{
+    float z = 0.0f;
+    const int64_t label = load_label(p.labels, p.label_bytes, row);
+    if (label >= 0 && label < p.vocab) {
+        const uint4 *a = static_cast<const uint4 *>(p.x) + static_cast<size_t>(row) * (p.width / 8);
+        const uint4 *b = static_cast<const uint4 *>(p.weight) + static_cast<size_t>(label) * (p.width / 8);
+#pragma unroll 5
+        for (int i = lane; i < p.width / 8; i += 32)
+            z = dot16<kBf16>(__ldg(a + i), __ldg(b + i), z);
     }
-    const double lse = static_cast<double>(mx) * 0.69314718055994530942 + log(static_cast<double>(sum));
-    p.lse[row] = static_cast<float>(lse);
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        z += __shfl_xor_sync(0xffffffffu, z, o);
+    return z;
+}
+
+// One row's loss and lse from its merged maximum, sum and target product.  In 64 bits: the
+// loss is a difference of terms near log(V).
+__device__ __forceinline__ void write_row(const Combine &p, int row, float mx, float sum, double target, float label_z)
+{
+    double lse = static_cast<double>(mx) * 0.69314718055994530942 + log(static_cast<double>(sum));
     double loss = 0.0;
     if (p.row_terms) {
         const double2 terms = p.row_terms[row];
@@ -888,14 +981,119 @@ __global__ void __launch_bounds__(32 * kCombineGroups) combine_kernel(const Comb
         }
     } else {
         const int64_t label = load_label(p.labels, p.label_bytes, row);
-        if (label != p.ignore_index) {
-            if (label >= 0 && label < p.vocab)
-                loss = lse - static_cast<double>(p.label_z[row]);
-            else
-                g_token_error = 1;
+        if (label >= 0 && label < p.vocab) {
+            const double formed = p.label_z[row];
+            lse -= exp(formed - lse) * (formed - label_z);
+            if (label != p.ignore_index)
+                loss = lse - label_z;
+        } else if (label != p.ignore_index) {
+            g_token_error = 1;
         }
     }
+    p.lse[row] = static_cast<float>(lse);
     p.losses[row] = static_cast<float>(loss);
+}
+
+constexpr int kBatch = 8; // partial results of a thread in flight together
+
+// Merges tiles first, first + step, ... of a row.
+__device__ __forceinline__ void merge_tiles(const Combine &p, int row, int first, int step, float &mx, float &sum,
+                                            double &target)
+{
+    for (; first < p.slices; first += kBatch * step) {
+        float m[kBatch], v[kBatch], t[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int i = first + j * step;
+            m[j] = -INFINITY;
+            v[j] = t[j] = 0.0f;
+            if (i < p.slices) {
+                const size_t at = static_cast<size_t>(i) * p.rows + row;
+                m[j] = __ldg(p.part_max + at);
+                v[j] = __ldg(p.part_sum + at);
+                if (p.part_t)
+                    t[j] = __ldg(p.part_t + at);
+            }
+        }
+        float next = mx;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            next = fmaxf(next, m[j]);
+        sum *= mx == -INFINITY ? 0.0f : exp2f(mx - next);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (first + j * step < p.slices)
+                sum = fmaf(v[j], exp2f(m[j] - next), sum);
+            target += t[j];
+        }
+        mx = next;
+    }
+}
+
+// Merges (mx, sum, target) with another; an empty side (maximum -infinity, sum 0) adds nothing.
+__device__ __forceinline__ void merge_pair(float &mx, float &sum, double &target, float m, float s, double t)
+{
+    const float next = fmaxf(mx, m);
+    sum = (mx == -INFINITY && sum == 0.0f ? 0.0f : sum * exp2f(mx - next)) +
+          (m == -INFINITY && s == 0.0f ? 0.0f : s * exp2f(m - next));
+    mx = next;
+    target += t;
+}
+
+// Forward's last step, in a fixed order.  Many rows: 32 rows per block, lane = row (coalesced),
+// warps over the column tiles.
+constexpr int kCombineGroups = 32;
+template <bool kBf16>
+__global__ void __launch_bounds__(32 * kCombineGroups) combine_kernel(const Combine p)
+{
+    __shared__ float s_max[kCombineGroups][32], s_sum[kCombineGroups][32];
+    __shared__ double s_t[kCombineGroups][32];
+    __shared__ float s_label[32];
+    griddepcontrol_wait();
+    griddepcontrol_launch_dependents();
+    const int group = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int row = blockIdx.x * 32 + lane;
+    float mx = -INFINITY, sum = 0.0f;
+    double target = 0.0;
+    if (row < p.rows)
+        merge_tiles(p, row, group, kCombineGroups, mx, sum, target);
+    s_max[group][lane] = mx;
+    s_sum[group][lane] = sum;
+    s_t[group][lane] = target;
+    const int mine = blockIdx.x * 32 + group; // this warp's row of the label products
+    if (p.labels && mine < p.rows) {
+        const float z = label_product<kBf16>(p, mine, lane);
+        if (lane == 0)
+            s_label[group] = z;
+    }
+    __syncthreads();
+    if (group != 0 || row >= p.rows)
+        return;
+    for (int i = 1; i < kCombineGroups && i < p.slices; ++i)
+        merge_pair(mx, sum, target, s_max[i][lane], s_sum[i][lane], s_t[i][lane]);
+    write_row(p, row, mx, sum, target, s_label[lane]);
+}
+
+// Few rows: a warp per row, lanes over the column tiles, so that every row's chain is short.
+constexpr int kCombineRowWarps = 4;
+template <bool kBf16>
+__global__ void __launch_bounds__(32 * kCombineRowWarps) combine_rows_kernel(const Combine p)
+{
+    griddepcontrol_wait();
+    griddepcontrol_launch_dependents();
+    const int row = blockIdx.x * kCombineRowWarps + threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (row >= p.rows)
+        return;
+    float mx = -INFINITY, sum = 0.0f;
+    double target = 0.0;
+    const float label_z = p.labels ? label_product<kBf16>(p, row, lane) : 0.0f;
+    merge_tiles(p, row, lane, 32, mx, sum, target);
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        merge_pair(mx, sum, target, __shfl_down_sync(0xffffffffu, mx, o), __shfl_down_sync(0xffffffffu, sum, o),
+                   __shfl_down_sync(0xffffffffu, target, o));
+    if (lane == 0)
+        write_row(p, row, mx, sum, target, label_z);
 }
 
 // dx = sum of the fp32 planes (one per K split), in order, times 1 / s: eight elements per thread.
@@ -931,13 +1129,30 @@ using namespace vocab;
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Up to this many rows one CTA per 128 x 128 tile of z is used instead of a pair per
-// 256 x 256: the rows fit one accumulator, W is streamed once, and narrow tiles spread it
-// over the SMs evenly.
+// Up to this many rows one CTA computes a tile instead of a pair: the rows fit one
+// accumulator and W is streamed once.
 constexpr int64_t kSingleRows = 128;
 
+// Up to this many rows the forward's last step takes a warp per row (20 rows: 10 us with 32
+// rows per block, TODO us with a warp each); above, its strided reads cost more than they save.
+constexpr int64_t kCombineRows = 1024;
+
 // Bytes of one piece of G.
-constexpr int64_t kPieceBytes = int64_t{256} << 20;
+constexpr int64_t kPieceBytes = int64_t{512} << 20;
+
+// Calls f with the entries per lane (1, 2, 4 or 8) that hold `targets` entries in a warp.
+template <class F>
+cudaError_t per_lane(int targets, F f)
+{
+    static_assert(kVocabMaxTargets == 256, "eight entries per lane, and entry numbers of 8 bits in the sort keys");
+    if (targets <= 32)
+        return f(std::integral_constant<int, 1>{});
+    if (targets <= 64)
+        return f(std::integral_constant<int, 2>{});
+    if (targets <= 128)
+        return f(std::integral_constant<int, 4>{});
+    return f(std::integral_constant<int, 8>{});
+}
 
 struct Arena {
     uint8_t *base;
@@ -951,10 +1166,38 @@ struct Arena {
     }
 };
 
+// Width of the equal tiles (multiples of 32) that cover `columns`.
+int even_width(int64_t columns)
+{
+    return static_cast<int>(round_up(ceil_div(columns, ceil_div(columns, kMaxBN)), 32));
+}
+
+// Width of z's tiles over `columns`: the one that finishes first, by rounds of the persistent
+// CTAs times a tile's time, which grows with its width, a fixed part for A's reads (about 32
+// columns' worth) and its start and epilogue (about three K blocks of 256).  20 x 51866: 295
+// tiles of 176 for 148 SMs, where 203 of 256 would leave the second round half empty.
+int logits_width(int64_t rows, int64_t columns, int64_t width, bool single, int align)
+{
+    const int64_t units = single ? sm_count() : sm_count() / 2;
+    const int64_t m_tiles = ceil_div(rows, single ? kBM : 2 * kBM);
+    const int64_t kbs = ceil_div(width, kBK);
+    int best = kMaxBN;
+    int64_t best_cost = INT64_MAX;
+    for (int bn = kMaxBN; bn >= 128; bn -= align) {
+        const int64_t rounds = ceil_div(m_tiles * ceil_div(columns, bn), units);
+        const int64_t cost = rounds * (kbs * (bn + 32) + 3 * 288);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = bn;
+        }
+    }
+    return best;
+}
+
 struct ForwardPlan {
     bool single;
-    int slice;
-    int64_t slices;
+    int bn;
+    int64_t slices; // column tiles
     float *part_max, *part_sum, *part_t, *label_z, *t_prob;
     int32_t *t_index;
     double2 *row_terms;
@@ -966,8 +1209,8 @@ ForwardPlan plan_forward(const VocabLossLaunch &L, void *workspace)
     ForwardPlan f{};
     Arena arena{static_cast<uint8_t *>(workspace)};
     f.single = L.rows <= kSingleRows;
-    f.slice = f.single ? 64 : 128;
-    f.slices = ceil_div(L.vocab, f.slice);
+    f.bn = logits_width(L.rows, L.vocab, L.width, f.single, f.single ? 16 : 32);
+    f.slices = ceil_div(L.vocab, f.bn);
     f.part_max = arena.take<float>(f.slices * L.rows);
     f.part_sum = arena.take<float>(f.slices * L.rows);
     if (L.targets > 0) {
@@ -987,7 +1230,7 @@ struct BackwardPlan {
     int targets;
     int64_t piece, pieces;   // vocabulary columns per piece of G
     int64_t ldg;             // elements per row of a piece
-    int dx_bn, dw_bn;
+    int grad_bn, width_bn;   // tile widths over a piece's columns, and over x's width
     int64_t splits;          // K splits of dx
     bool planes;
     float *row_lse2, *row_gain, *inv_gain, *t_prob, *dx_planes;
@@ -996,8 +1239,33 @@ struct BackwardPlan {
     int64_t bytes;
 };
 
-// A 128-wide tile where it saves a whole half tile of padding.
-int tile_width(int64_t columns) { return columns % 256 != 0 && columns % 256 <= 128 ? 128 : 256; }
+// K splits of dx = G W, whose tiles (rows x width) are few while its K axis, a piece of the
+// vocabulary, is long.  The splits that finish first by a count of K blocks: rounds of the
+// persistent CTAs times a tile's blocks (and about four for its start and epilogue), plus the
+// fp32 planes' write and read at 1.6 MB per block's time (0.33 us at 5 TB/s).  3584 x 768 x
+// 51865: 42 tiles for 74 pairs, one split 265 us, three splits 190 us with their planes.
+int64_t dx_splits(const VocabLossLaunch &L, const BackwardPlan &b)
+{
+    const int64_t units = b.single ? sm_count() : sm_count() / 2;
+    const int64_t tiles = ceil_div(L.rows, b.single ? kBM : 2 * kBM) * ceil_div(L.width, b.width_bn);
+    const int64_t kbs = ceil_div(b.piece, kBK);
+    int64_t best = 1;
+    double best_cost = INFINITY;
+    for (int64_t s = 1; s <= units; ++s) {
+        const int64_t per = ceil_div(kbs, s);
+        if (s > 1 && per < 4)
+            break;
+        const int64_t used = ceil_div(kbs, per);
+        const bool planes = used > 1 || b.pieces > 1;
+        const double cost = static_cast<double>(ceil_div(tiles * used, units) * (per + 4)) * b.pieces +
+                            (planes ? static_cast<double>(used) * L.rows * L.width * 8 / 1.6e6 : 0.0);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = used;
+        }
+    }
+    return best;
+}
 
 BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
 {
@@ -1010,13 +1278,9 @@ BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
     b.piece = std::min(L.vocab, round_up(ceil_div(L.vocab, b.pieces), 256));
     b.pieces = ceil_div(L.vocab, b.piece);
     b.ldg = round_up(b.piece, 64);
-    b.dx_bn = b.single ? 128 : tile_width(L.width);
-    b.dw_bn = tile_width(L.width);
-    const int64_t units = b.single ? sm_count() : sm_count() / 2;
-    const int64_t tiles = ceil_div(L.rows, b.single ? kBM : 2 * kBM) * ceil_div(L.width, b.dx_bn);
-    const int64_t kbs = ceil_div(b.piece, kBK);
-    const int64_t want = std::max<int64_t>(1, std::min(units / std::max<int64_t>(tiles, 1), kbs / 4));
-    b.splits = ceil_div(kbs, ceil_div(kbs, want));
+    b.grad_bn = logits_width(L.rows, b.piece, L.width, b.single, 32);
+    b.width_bn = even_width(L.width);
+    b.splits = dx_splits(L, b);
     b.planes = b.splits > 1 || b.pieces > 1;
     b.row_lse2 = arena.take<float>(L.rows);
     b.row_gain = arena.take<float>(L.rows);
@@ -1039,6 +1303,11 @@ bool map16(CUtensorMap *map, bool bf16, const void *base, int64_t rows, int64_t 
                        cols, ld, static_cast<uint32_t>(box_cols), static_cast<uint32_t>(box_rows), swizzle);
 }
 
+// Rows of an A tile that are loaded.  Few rows (one CTA's tile) are loaded as such: the rest of
+// the tile keeps what shared memory held, and only rows of the accumulator that nothing reads
+// are computed from it.
+int tile_rows(int64_t rows) { return static_cast<int>(rows < kBM ? round_up(rows, 8) : kBM); }
+
 // An operand of a GEMM: K-major ([mn, k] in memory) or MN-major ([k, mn]).
 bool operand_map(CUtensorMap *map, bool bf16, bool mn_major, const void *base, int64_t rows, int64_t cols, int64_t ld,
                  int mn_rows)
@@ -1047,12 +1316,13 @@ bool operand_map(CUtensorMap *map, bool bf16, bool mn_major, const void *base, i
                     : map16(map, bf16, base, rows, cols, ld, kBK, mn_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int BN, bool kPair, int MODE, bool kBf16, bool kPlanes>
+// p: m, n, bn and num_kb, kb_per set.
+template <bool kPair, int MODE, bool kBf16, bool kPlanes>
 cudaError_t launch_one(const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &out, Params p,
                        cudaStream_t stream)
 {
-    using C = Cfg<BN, kPair, MODE>;
-    auto kernel = gemm_kernel<BN, kPair, MODE, kBf16, kPlanes>;
+    using C = Cfg<kPair, MODE>;
+    auto kernel = gemm_kernel<kPair, MODE, kBf16, kPlanes>;
     static std::atomic<bool> opted[kMaxDevices];
     const int device = current_device();
     if (!opted[device].load(std::memory_order_acquire)) {
@@ -1063,10 +1333,11 @@ cudaError_t launch_one(const CUtensorMap &a, const CUtensorMap &b, const CUtenso
         opted[device].store(true, std::memory_order_release);
     }
     p.m_tiles = static_cast<int>(ceil_div(p.m, C::kTileM));
-    p.n_tiles = static_cast<int>(ceil_div(p.n, BN));
+    p.n_tiles = static_cast<int>(ceil_div(p.n, p.bn));
     const int64_t splits = ceil_div(p.num_kb, p.kb_per);
     p.num_tiles = static_cast<int>(splits * p.m_tiles * p.n_tiles);
-    p.type_bits = kBf16 ? (1u << 7) | (1u << 10) : 0u;
+    p.a_rows = tile_rows(p.m);
+    p.idesc_bits = (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (static_cast<uint32_t>(p.bn >> 3) << 17);
     const int units = kPair ? sm_count() / 2 : sm_count();
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(std::min(p.num_tiles, units) * (kPair ? 2 : 1)));
@@ -1092,21 +1363,22 @@ cudaError_t launch_one(const CUtensorMap &a, const CUtensorMap &b, const CUtenso
 
 // z tiles: x [rows, width] times columns [col0, col0 + cols) of W^T.
 template <int MODE, bool kBf16>
-cudaError_t launch_logits(const VocabLossLaunch &L, const void *x, int64_t col0, int64_t cols, bool single,
+cudaError_t launch_logits(const VocabLossLaunch &L, const void *x, int64_t col0, int64_t cols, int bn, bool single,
                           const CUtensorMap &out, Params p, cudaStream_t stream)
 {
     CUtensorMap a, b;
     const uint16_t *w = static_cast<const uint16_t *>(L.weight) + col0 * L.width;
-    if (!operand_map(&a, kBf16, false, x, L.rows, L.width, L.width, kBM) ||
-        !operand_map(&b, kBf16, false, w, cols, L.width, L.width, 128))
+    if (!operand_map(&a, kBf16, false, x, L.rows, L.width, L.width, tile_rows(L.rows)) ||
+        !operand_map(&b, kBf16, false, w, cols, L.width, L.width, single ? bn : bn / 2))
         return cudaErrorInvalidValue;
     p.m = static_cast<int>(L.rows);
     p.n = static_cast<int>(cols);
+    p.bn = bn;
     p.col0 = static_cast<int>(col0);
     p.num_kb = p.kb_per = static_cast<int>(ceil_div(L.width, kBK));
     p.scale2 = static_cast<float>(1.4426950408889634 / static_cast<double>(L.temperature));
-    return single ? launch_one<128, false, MODE, kBf16, false>(a, b, out, p, stream)
-                  : launch_one<256, true, MODE, kBf16, false>(a, b, out, p, stream);
+    return single ? launch_one<false, MODE, kBf16, false>(a, b, out, p, stream)
+                  : launch_one<true, MODE, kBf16, false>(a, b, out, p, stream);
 }
 
 template <bool kBf16>
@@ -1127,8 +1399,10 @@ cudaError_t run_forward(const VocabLossLaunch &L, cudaStream_t stream)
         t.index = f.t_index;
         t.prob = f.t_prob;
         const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, kPrepWarps), 8 * sm_count());
-        err = launch_pdl(targets_kernel, dim3(static_cast<unsigned>(blocks)), dim3(32 * kPrepWarps), stream, t,
-                         f.row_terms);
+        err = per_lane(L.targets, [&](auto r) {
+            return launch_pdl(targets_kernel<decltype(r)::value>, dim3(static_cast<unsigned>(blocks)),
+                              dim3(32 * kPrepWarps), stream, t, f.row_terms);
+        });
         if (err != cudaSuccess)
             return err;
         p.t_index = f.t_index;
@@ -1141,25 +1415,31 @@ cudaError_t run_forward(const VocabLossLaunch &L, cudaStream_t stream)
     p.part_sum = f.part_sum;
     p.part_t = f.part_t;
     p.label_z = f.label_z;
-    err = launch_logits<kStats, kBf16>(L, L.x, 0, L.vocab, f.single, CUtensorMap{}, p, stream);
+    err = launch_logits<kStats, kBf16>(L, L.x, 0, L.vocab, f.bn, f.single, CUtensorMap{}, p, stream);
     if (err != cudaSuccess)
         return err;
     Combine c{};
     c.rows = static_cast<int>(L.rows);
     c.slices = static_cast<int>(f.slices);
     c.vocab = static_cast<int>(L.vocab);
+    c.width = static_cast<int>(L.width);
+    c.x = L.x;
+    c.weight = L.weight;
     c.part_max = f.part_max;
     c.part_sum = f.part_sum;
     c.part_t = f.part_t;
     c.label_z = f.label_z;
-    c.labels = L.labels;
+    c.labels = L.targets > 0 ? nullptr : L.labels;
     c.label_bytes = L.label_bytes;
     c.ignore_index = L.ignore_index;
     c.row_terms = f.row_terms;
     c.temperature = L.temperature;
     c.losses = L.losses;
     c.lse = L.lse_out;
-    return launch_pdl(combine_kernel, dim3(static_cast<unsigned>(ceil_div(L.rows, 32))), dim3(32 * kCombineGroups),
+    if (L.rows <= kCombineRows)
+        return launch_pdl(combine_rows_kernel<kBf16>, dim3(static_cast<unsigned>(ceil_div(L.rows, kCombineRowWarps))),
+                          dim3(32 * kCombineRowWarps), stream, c);
+    return launch_pdl(combine_kernel<kBf16>, dim3(static_cast<unsigned>(ceil_div(L.rows, 32))), dim3(32 * kCombineGroups),
                       stream, c);
 }
 
@@ -1169,15 +1449,15 @@ cudaError_t launch_dx(const VocabLossLaunch &L, const BackwardPlan &b, int64_t c
 {
     CUtensorMap ma, mb, out;
     const uint16_t *w = static_cast<const uint16_t *>(L.weight) + col0 * L.width;
-    if (!operand_map(&ma, kBf16, false, b.g, L.rows, cols, b.ldg, kBM) ||
+    if (!operand_map(&ma, kBf16, false, b.g, L.rows, cols, b.ldg, tile_rows(L.rows)) ||
         !operand_map(&mb, kBf16, true, w, cols, L.width, L.width, 0))
         return cudaErrorInvalidValue;
     if (b.planes) {
         const int64_t dims[3] = {L.width, L.rows, b.splits};
         const int64_t strides[2] = {L.width * 4, L.rows * L.width * 4};
-        const uint32_t box[3] = {kSub, 32u, 1u};
+        const uint32_t box[3] = {16u, 32u, 1u};
         if (!make_map_nd(&out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, b.dx_planes, dims, strides, box,
-                         CU_TENSOR_MAP_SWIZZLE_128B))
+                         CU_TENSOR_MAP_SWIZZLE_64B))
             return cudaErrorInvalidValue;
     } else if (!map16(&out, kBf16, L.dx, L.rows, L.width, L.width, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
         return cudaErrorInvalidValue;
@@ -1187,19 +1467,15 @@ cudaError_t launch_dx(const VocabLossLaunch &L, const BackwardPlan &b, int64_t c
     p.n = static_cast<int>(L.width);
     p.num_kb = static_cast<int>(ceil_div(cols, kBK));
     p.kb_per = static_cast<int>(ceil_div(ceil_div(b.piece, kBK), b.splits));
+    p.bn = b.width_bn;
     p.n_first = 1;
     p.inv_gain = b.inv_gain;
     p.accumulate = first ? 0 : 1;
-    if (b.planes) {
-        if (b.single)
-            return launch_one<128, false, kDx, kBf16, true>(ma, mb, out, p, stream);
-        return b.dx_bn == 128 ? launch_one<128, true, kDx, kBf16, true>(ma, mb, out, p, stream)
-                              : launch_one<256, true, kDx, kBf16, true>(ma, mb, out, p, stream);
-    }
-    if (b.single)
-        return launch_one<128, false, kDx, kBf16, false>(ma, mb, out, p, stream);
-    return b.dx_bn == 128 ? launch_one<128, true, kDx, kBf16, false>(ma, mb, out, p, stream)
-                          : launch_one<256, true, kDx, kBf16, false>(ma, mb, out, p, stream);
+    if (b.planes)
+        return b.single ? launch_one<false, kDx, kBf16, true>(ma, mb, out, p, stream)
+                        : launch_one<true, kDx, kBf16, true>(ma, mb, out, p, stream);
+    return b.single ? launch_one<false, kDx, kBf16, false>(ma, mb, out, p, stream)
+                    : launch_one<true, kDx, kBf16, false>(ma, mb, out, p, stream);
 }
 
 template <bool kBf16>
@@ -1216,10 +1492,10 @@ cudaError_t launch_dw(const VocabLossLaunch &L, const BackwardPlan &b, int64_t c
     p.m = static_cast<int>(cols);
     p.n = static_cast<int>(L.width);
     p.num_kb = p.kb_per = static_cast<int>(ceil_div(L.rows, kBK));
+    p.bn = b.width_bn;
     p.n_first = 1;
     p.inv_gain = b.inv_gain;
-    return b.dw_bn == 128 ? launch_one<128, true, kDw, kBf16, false>(ma, mb, out, p, stream)
-                          : launch_one<256, true, kDw, kBf16, false>(ma, mb, out, p, stream);
+    return launch_one<true, kDw, kBf16, false>(ma, mb, out, p, stream);
 }
 
 template <bool kBf16>
@@ -1249,8 +1525,13 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
     q.row_gain = b.row_gain;
     q.inv_gain = b.inv_gain;
     const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, kPrepWarps), 4 * sm_count());
-    cudaError_t err =
-        launch_pdl(prepare_kernel, dim3(static_cast<unsigned>(blocks)), dim3(32 * kPrepWarps), stream, q);
+    const dim3 grid(static_cast<unsigned>(blocks)), block(32 * kPrepWarps);
+    cudaError_t err = L.targets > 0 ? per_lane(L.targets,
+                                               [&](auto r) {
+                                                   return launch_pdl(prepare_kernel<decltype(r)::value>, grid, block,
+                                                                     stream, q);
+                                               })
+                                    : launch_pdl(prepare_kernel<0>, grid, block, stream, q);
     if (err != cudaSuccess)
         return err;
     for (int64_t col0 = 0; col0 < L.vocab; col0 += b.piece) {
@@ -1264,7 +1545,7 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
         p.targets = b.targets;
         p.row_lse2 = b.row_lse2;
         p.row_gain = b.row_gain;
-        err = launch_logits<kGrad, kBf16>(L, b.x_masked, col0, cols, b.single, out, p, stream);
+        err = launch_logits<kGrad, kBf16>(L, b.x_masked, col0, cols, b.grad_bn, b.single, out, p, stream);
         if (err == cudaSuccess && L.dx)
             err = launch_dx<kBf16>(L, b, col0, cols, col0 == 0, stream);
         if (err == cudaSuccess && L.dweight)
@@ -1274,8 +1555,8 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
     }
     if (L.dx && b.planes) {
         const int64_t elements = L.rows * L.width;
-        const int64_t grid = std::min<int64_t>(ceil_div(elements / 8, 256), 8 * sm_count());
-        err = launch_pdl(planes_kernel<kBf16>, dim3(static_cast<unsigned>(grid)), dim3(256), stream,
+        const int64_t plane_blocks = std::min<int64_t>(ceil_div(elements / 8, 256), 8 * sm_count());
+        err = launch_pdl(planes_kernel<kBf16>, dim3(static_cast<unsigned>(plane_blocks)), dim3(256), stream,
                          static_cast<const float *>(b.dx_planes), static_cast<int>(b.splits),
                          static_cast<size_t>(elements), static_cast<const float *>(b.inv_gain),
                          static_cast<uint4 *>(L.dx));

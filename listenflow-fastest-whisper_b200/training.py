@@ -64,8 +64,15 @@ def _vector(t: torch.Tensor, dtypes, count: int, device: torch.device, name: str
         raise ValueError(f"{name} must be a contiguous {kinds} tensor [{count}] on {device}")
 
 
+# The current stream's handle by device index, without a Stream object around it (a tenth of
+# a small call's host time).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _run(call, args, name: str, device: torch.device) -> None:
-    native.check(call(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream), name)
+    status = call(ctypes.byref(args), _raw_stream(device.index))
+    if status:
+        native.check(status, name)
 
 
 _FLOAT = (torch.float32,)
@@ -89,7 +96,7 @@ def layer_norm_forward(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor,
     with _scope(device, stream):
         total = x if residual is None else torch.empty_like(x)
         y = torch.empty_like(x)
-        stats = torch.empty((2, rows), dtype=torch.float32, device=device)
+        stats = gamma.new_empty((2, rows))
         if rows:
             a = native.LayerNormTrainArgs(
                 ctypes.sizeof(native.LayerNormTrainArgs), rows, cols, dtype, x.data_ptr(),
@@ -122,18 +129,18 @@ def layer_norm_backward(dy: torch.Tensor, total: torch.Tensor, gamma: torch.Tens
         dgamma = dbeta = workspace = None
         size = 0
         if not rows:
-            zeros = (lambda: torch.zeros(cols, dtype=torch.float32, device=device)) if want_params else (lambda: None)
-            return dx, zeros(), zeros()
+            return (dx, torch.zeros_like(gamma), torch.zeros_like(gamma)) if want_params else (dx, None, None)
         lib = native.library()
         if want_params:
-            dgamma = torch.empty(cols, dtype=torch.float32, device=device)
-            dbeta = torch.empty(cols, dtype=torch.float32, device=device)
+            dgamma, dbeta = gamma.new_empty(cols), gamma.new_empty(cols)
             size = lib.lffw_layer_norm_grad_workspace(rows, cols)
-            workspace = torch.empty(size, dtype=torch.uint8, device=device)
-        ptr = lambda t: None if t is None else t.data_ptr()
+            if size > 0:
+                workspace = gamma.new_empty(size // 4)
         a = native.LayerNormGradArgs(
             ctypes.sizeof(native.LayerNormGradArgs), rows, cols, dtype, dy.data_ptr(), total.data_ptr(),
-            gamma.data_ptr(), stats.data_ptr(), ptr(dsum), ptr(dx), ptr(dgamma), ptr(dbeta), ptr(workspace), size)
+            gamma.data_ptr(), stats.data_ptr(), None if dsum is None else dsum.data_ptr(),
+            dx.data_ptr() if want_dx else None, dgamma.data_ptr() if want_params else None,
+            dbeta.data_ptr() if want_params else None, None if workspace is None else workspace.data_ptr(), size)
         _run(lib.lffw_layer_norm_grad, a, "lffw_layer_norm_grad", device)
     return dx, dgamma, dbeta
 
@@ -144,24 +151,22 @@ def layer_norm_backward(dy: torch.Tensor, total: torch.Tensor, gamma: torch.Tens
 def _operands(x: torch.Tensor, weight: torch.Tensor) -> native.VocabLossArgs:
     dtype = _rows(x, "x")
     _rows(weight, "weight")
-    if weight.dtype != x.dtype or weight.device != x.device or weight.shape[1] != x.shape[1] or not weight.shape[0]:
+    (rows, width), (vocab, weight_width) = x.shape, weight.shape
+    if weight.dtype != x.dtype or weight.device != x.device or weight_width != width or not vocab:
         raise ValueError("weight must be [vocab, width] of x's type and device")
-    a = native.VocabLossArgs()
-    a.struct_size = ctypes.sizeof(native.VocabLossArgs)
-    a.rows, a.width, a.vocab, a.dtype = x.shape[0], x.shape[1], weight.shape[0], dtype
-    a.x, a.weight = x.data_ptr(), weight.data_ptr()
-    return a
+    return native.VocabLossArgs(ctypes.sizeof(native.VocabLossArgs), rows, width, vocab, dtype, x.data_ptr(),
+                                weight.data_ptr())
 
 
 def _with_labels(a: native.VocabLossArgs, x: torch.Tensor, labels: torch.Tensor, ignore_index: int) -> None:
-    _vector(labels, _LABELS, x.shape[0], x.device, "labels")
+    _vector(labels, _LABELS, a.rows, x.device, "labels")
     a.labels, a.label_bytes, a.ignore_index = labels.data_ptr(), labels.element_size(), ignore_index
     a.temperature = 1.0
 
 
 def _with_teacher(a: native.VocabLossArgs, x: torch.Tensor, tokens: torch.Tensor, logits: torch.Tensor,
                   temperature: float) -> None:
-    if (tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != x.shape[0]
+    if (tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != a.rows
             or not 1 <= tokens.shape[1] <= MAX_TEACHER_ENTRIES or tokens.device != x.device
             or not tokens.is_contiguous()):
         raise ValueError(f"teacher_tokens must be a contiguous int32 tensor [rows, 1 to {MAX_TEACHER_ENTRIES}] "
@@ -175,41 +180,44 @@ def _with_teacher(a: native.VocabLossArgs, x: torch.Tensor, tokens: torch.Tensor
     a.teacher_tokens, a.teacher_logits, a.temperature = tokens.data_ptr(), logits.data_ptr(), temperature
 
 
+def _workspace(a: native.VocabLossArgs, x: torch.Tensor, grad: int) -> torch.Tensor:
+    size = native.library().lffw_vocab_loss_workspace(ctypes.byref(a), grad)
+    if size < 0:
+        native.check(native.INVALID_ARGUMENT, "lffw_vocab_loss_workspace")
+    workspace = x.new_empty((size + 1) // 2)
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), size
+    return workspace
+
+
 def _loss_forward(a: native.VocabLossArgs, x: torch.Tensor, stream):
-    device = x.device
+    device, rows = x.device, a.rows
     with _scope(device, stream):
-        losses = torch.empty(a.rows, dtype=torch.float32, device=device)
-        lse = torch.empty(a.rows, dtype=torch.float32, device=device)
-        if a.rows:
-            lib = native.library()
+        losses = torch.empty(rows, dtype=torch.float32, device=device)
+        lse = torch.empty_like(losses)
+        if rows:
             a.losses, a.lse = losses.data_ptr(), lse.data_ptr()
-            a.workspace_bytes = lib.lffw_vocab_loss_workspace(ctypes.byref(a), 0)
-            workspace = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=device)
-            a.workspace = workspace.data_ptr()
-            _run(lib.lffw_vocab_loss, a, "lffw_vocab_loss", device)
+            workspace = _workspace(a, x, 0)  # noqa: F841 (freed after the call is queued)
+            _run(native.library().lffw_vocab_loss, a, "lffw_vocab_loss", device)
     return losses, lse
 
 
 def _loss_backward(a: native.VocabLossArgs, x: torch.Tensor, weight: torch.Tensor, lse: torch.Tensor,
                    dloss: torch.Tensor, want_dx: bool, want_dweight: bool, stream):
-    device = x.device
-    _vector(lse, _FLOAT, x.shape[0], device, "lse")
-    _vector(dloss, _FLOAT, x.shape[0], device, "dloss")
+    device, rows = x.device, a.rows
+    _vector(lse, _FLOAT, rows, device, "lse")
+    _vector(dloss, _FLOAT, rows, device, "dloss")
     if not want_dx and not want_dweight:
         raise ValueError("nothing to compute: want_dx and want_dweight are both false")
     with _scope(device, stream):
         dx = torch.empty_like(x) if want_dx else None
-        if not a.rows:
+        if not rows:
             return dx, torch.zeros_like(weight) if want_dweight else None
         dweight = torch.empty_like(weight) if want_dweight else None
-        lib = native.library()
         a.lse, a.dloss = lse.data_ptr(), dloss.data_ptr()
         a.dx = dx.data_ptr() if want_dx else None
         a.dweight = dweight.data_ptr() if want_dweight else None
-        a.workspace_bytes = lib.lffw_vocab_loss_workspace(ctypes.byref(a), 1)
-        workspace = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=device)
-        a.workspace = workspace.data_ptr()
-        _run(lib.lffw_vocab_loss_grad, a, "lffw_vocab_loss_grad", device)
+        workspace = _workspace(a, x, 1)  # noqa: F841 (freed after the call is queued)
+        _run(native.library().lffw_vocab_loss_grad, a, "lffw_vocab_loss_grad", device)
     return dx, dweight
 
 
