@@ -7,16 +7,18 @@
 //            (one target with t = 1 and T = 1: lse_i - z_i,label)
 //   gradient G_iv = g_i T (exp(z_iv / T - lse_i) - t_iv),  dx = G W,  dW = G^T x
 //
-// Everything of size n x V runs through one tensor-core GEMM kernel in four forms:
+// Everything of size n x V runs through one tensor-core GEMM kernel in three forms:
 //   kStats   z tiles, reduced in the epilogue to a running maximum, a sum of exponentials and
 //            the targets' logits per row and column slice (merged by combine_kernel)
 //   kGrad    z tiles again, turned in the epilogue into a piece of G (16 bits, a range of
 //            vocabulary columns)
-//   kDx      that piece times its rows of W, summed over the pieces in fp32
-//   kDw      that piece transposed times x: its rows of dW
+//   kBack    that piece times its rows of W (dx, summed over the pieces in fp32) and that piece
+//            transposed times x (its rows of dW), one list of tiles shared out over the SMs
 // A piece of G is the only n x (part of V) tensor that ever exists.
 //
-// The work is bound by the tensor cores (2 n V d flops per form, four forms for a training
+// Rows without a target are left out of the gradients' products altogether (labels).
+//
+// The work is bound by the tensor cores (2 n V d flops per product, four products in a training
 // step: the logits are formed twice because they are not kept) once n exceeds a few hundred
 // rows; below that it is bound by streaming W (and writing dW).
 #include <cuda.h>
@@ -41,13 +43,11 @@ namespace vocab {
 constexpr int kBM = 128;               // accumulator rows per CTA (TMEM lanes)
 constexpr int kBK = 64;                // K elements per stage: one 128-byte swizzle row
 constexpr int kUmmaK = 16;             // K of one kind::f16 MMA
-constexpr int kEpiWarps = 16;          // four per TMEM lane quarter, each with a quarter of the tile's columns
-constexpr int kThreads = 64 + 32 * kEpiWarps; // warp 0 TMA, warp 1 MMA, warps 2-17 epilogue
 constexpr int kSub = 32;               // columns per epilogue step
 constexpr int kMaxBN = 256;            // widest tile
 constexpr float kLog2e = 1.4426950408889634f;
 
-enum Mode : int { kStats, kGrad, kDx, kDw };
+enum Mode : int { kStats, kGrad, kBack };
 
 // A label or a teacher token outside the vocabulary was met (see lffw_vocab_loss_error).
 __device__ int g_token_error = 0;
@@ -65,15 +65,21 @@ __device__ int g_token_error = 0;
 // many as the SMs share evenly.
 template <bool kPair, int MODE>
 struct Cfg {
-    static constexpr bool kAMn = MODE == kDw;
-    static constexpr bool kBMn = MODE == kDx || MODE == kDw;
+    // Epilogue warps: per TMEM lane quarter two, each with half of a tile's columns, or four.
+    // kGrad, whose epilogue is the longest, gains from sixteen where K is short (384: 24.8 ->
+    // 22.3 us for 333 rows); the others are as fast or faster with eight (7168 x 1280 kStats
+    // 634 -> 623 us).
+    static constexpr int kEpiWarps = MODE == kGrad ? 16 : 8;
+    static constexpr int kParts = kEpiWarps / 4;
+    static constexpr int kThreads = 64 + 32 * kEpiWarps; // warp 0 TMA, warp 1 MMA, then the epilogue
     static constexpr int kTileM = kPair ? 2 * kBM : kBM;
     static constexpr int kABytes = kBM * 128;
     static constexpr int kBBytes = (kPair ? kMaxBN / 2 : kMaxBN) * 128; // this CTA's rows of B, at most
     static constexpr int kStageBytes = kABytes + kBBytes;
     // Per epilogue warp: kStats exchanges (maximum, sum, target product) of 32 rows, twice
-    // (tile parity); the others stage a 32-row x 64-byte store.
-    static constexpr int kStaging = MODE == kStats ? 2 * 3 * 32 * 4 : 2048;
+    // (tile parity); the others stage 32-row x 64-byte stores.
+    static constexpr int kBuffers = 16 / kEpiWarps;
+    static constexpr int kStaging = MODE == kStats ? 2 * 3 * 32 * 4 : 2048 * kBuffers;
     static constexpr int kBarBytes = 256;
     static constexpr int kBudget = 232448 - 1024;
     static constexpr int kFit = (kBudget - kEpiWarps * kStaging - kBarBytes) / kStageBytes;
@@ -83,22 +89,23 @@ struct Cfg {
     static constexpr int kOffBar = kOffStaging + kEpiWarps * kStaging;
     static constexpr int kSmemBytes = kOffBar + kBarBytes + 1024;
     static constexpr int kTmemCols = 2 * kMaxBN; // two accumulators
-    // Instruction descriptor without its operand types and N.
-    static constexpr uint32_t kIdesc = (1u << 4) | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u) |
-                                       (static_cast<uint32_t>(kTileM >> 4) << 24);
+    // Instruction descriptor without its operand types, major axes and N.
+    static constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(kTileM >> 4) << 24);
     static_assert(kStages >= 4 && kSmemBytes <= 232448, "shared memory budget");
     static_assert((2 * kStages + 5) * 8 + 8 <= kBarBytes, "barrier area");
 };
 
+constexpr uint32_t kAMnMajor = 1u << 15, kBMnMajor = 1u << 16; // instruction descriptor bits
+
 struct Params {
-    int m, n;                    // rows and columns of the output
-    int m_tiles, n_tiles, num_tiles;
+    int rows;                    // token rows (the most there can be)
+    const int *rows_used;        // how many of them there are, on the device (null: all)
+    int n, n_tiles;              // output columns: the vocabulary's (kStats, kGrad), x's width (kBack)
     int bn;                      // tile width
-    int a_rows;                  // rows of a K-major A tile that are loaded (kBM, or few rows rounded up)
-    int num_kb, kb_per;          // K blocks, and how many of them one split sums
-    int n_first;                 // raster: 0 = M tiles fastest, 1 = N tiles fastest
+    int num_kb;                  // kStats, kGrad: K blocks (of x's width)
+    int a_rows;                  // token rows of a K-major A tile that are loaded (kBM, or few rows rounded up)
     uint32_t idesc_bits;         // instruction descriptor's operand types and N
-    // kStats and kGrad: row i is token i, column c is vocabulary entry col0 + c.
+    // kStats and kGrad: column c is vocabulary entry col0 + c.
     int col0;
     float scale2;                // log2(e) / T
     const void *labels;          // kStats, one target: int32 or int64 per row
@@ -106,12 +113,15 @@ struct Params {
     const int32_t *t_index;      // sorted target columns [rows, targets] (INT_MAX: none)
     const float *t_prob;
     int targets;
-    float *part_max, *part_sum, *part_t; // [slices, rows]; part_t holds sum_j t_j z_j
+    float *part_max, *part_sum, *part_t; // [column tiles, rows]; part_t holds sum_j t_j z_j
     float *label_z;              // kStats, one target: z of the label
     const float *row_lse2, *row_gain; // kGrad: lse log2(e), and g T s
-    // kDx and kDw
+    // kBack
+    int vocab;                   // the piece's vocabulary columns: K of dx, rows of dW
+    int dx_splits, dx_kb_per;    // K splits of dx (0: no dx) and their K blocks
+    int dw_tiles;                // tiles of dW (0: no dW)
+    int accumulate;              // add to the fp32 planes
     const float *inv_gain;       // 1 / s
-    int accumulate;              // kDx: add to the fp32 planes
 };
 
 __device__ __forceinline__ float exp2_approx(float x)
@@ -223,12 +233,13 @@ __device__ __forceinline__ uint64_t desc_mn_boxes(uint32_t addr)
     return desc;
 }
 
-// tm_a, tm_b: operands.  tm_out: G (kGrad), dW (kDw), dx itself or the fp32 planes (kDx).
-// Planes is the kDx form that writes fp32 planes instead of dx.
-template <bool kPair, int MODE, bool kBf16, bool kPlanes>
-__global__ void __launch_bounds__(kThreads, 1)
+// tm_a, tm_b, tm_out: operands and output (G) of kStats and kGrad; G, W and the fp32 planes of
+// dx in kBack.  tm_a2, tm_b2, tm_out2: G, x and dW of kBack.
+template <bool kPair, int MODE, bool kBf16>
+__global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                const __grid_constant__ CUtensorMap tm_out, const Params p)
+                const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ CUtensorMap tm_a2,
+                const __grid_constant__ CUtensorMap tm_b2, const __grid_constant__ CUtensorMap tm_out2, const Params p)
 {
     using C = Cfg<kPair, MODE>;
     extern __shared__ uint8_t smem_raw[];
@@ -240,34 +251,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int lane = threadIdx.x % 32;
     const uint32_t rank = kPair ? cluster_ctarank() : 0u;
     const bool leader = rank == 0;
-    const int tile_step = kPair ? static_cast<int>(gridDim.x / 2) : static_cast<int>(gridDim.x);
-    const int tile_first = kPair ? static_cast<int>(blockIdx.x / 2) : static_cast<int>(blockIdx.x);
+    const int units = kPair ? static_cast<int>(gridDim.x / 2) : static_cast<int>(gridDim.x);
+    const int unit = kPair ? static_cast<int>(blockIdx.x / 2) : static_cast<int>(blockIdx.x);
     const uint32_t bar_full = sbase + C::kOffBar;
     const uint32_t bar_empty = bar_full + 8 * C::kStages;
     const uint32_t bar_acc_full = bar_empty + 8 * C::kStages;
     const uint32_t bar_acc_empty = bar_acc_full + 16;
     const uint32_t bar_drain = bar_acc_empty + 16;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::kOffBar + (2 * C::kStages + 5) * 8);
-
-    struct Tile {
-        int m0, n0, kb0, kbn, split;
-    };
-    // Tile t: this CTA's first row, the tile's first column, and its K blocks.  A function of
-    // t alone: the producer, the MMA issuer and the epilogue agree.
-    auto tile_at = [&](int t) {
-        const int per_split = p.m_tiles * p.n_tiles;
-        const int split = t / per_split;
-        const int r = t - split * per_split;
-        const int mt = p.n_first ? r / p.n_tiles : r % p.m_tiles;
-        const int nt = p.n_first ? r % p.n_tiles : r / p.m_tiles;
-        Tile tile;
-        tile.m0 = mt * C::kTileM + static_cast<int>(rank) * kBM;
-        tile.n0 = nt * p.bn;
-        tile.split = split;
-        tile.kb0 = split * p.kb_per;
-        tile.kbn = min(p.kb_per, p.num_kb - tile.kb0);
-        return tile;
-    };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::kStages; ++s) {
@@ -276,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(bar_acc_full + 8 * a, 1);
-            mbar_init(bar_acc_empty + 8 * a, kPair ? 2 * kEpiWarps : kEpiWarps);
+            mbar_init(bar_acc_empty + 8 * a, kPair ? 2 * C::kEpiWarps : C::kEpiWarps);
         }
         mbar_init(bar_drain, 1);
         fence_barrier_init();
@@ -284,6 +275,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tensor_map(&tm_b);
         if (MODE != kStats)
             prefetch_tensor_map(&tm_out);
+        if (MODE == kBack) {
+            prefetch_tensor_map(&tm_a2);
+            prefetch_tensor_map(&tm_b2);
+            prefetch_tensor_map(&tm_out2);
+        }
     }
     if (warp == 1) {
         if (kPair) {
@@ -307,6 +303,64 @@ __global__ void __launch_bounds__(kThreads, 1)
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
 
+    const int rows = p.rows_used ? *p.rows_used : p.rows;
+    struct Tile {
+        int m0, n0, kb0, kbn, split;
+        bool dw;
+    };
+    // The i-th tile of this CTA (pair): its first row, the tile's first column and its K blocks;
+    // false past the last.  A function of i alone: the producer, the MMA issuer and the epilogue
+    // agree.
+    const int m_tiles = (rows + C::kTileM - 1) / C::kTileM;
+    // kBack: the dx tiles (long: K is the piece of the vocabulary) are dealt out first, the dW
+    // tiles (K: the rows) after them.  Where a last round of dx tiles leaves units without one,
+    // those take as many dW tiles more as fit into its time (in K blocks, a tile's start and
+    // epilogue counted as six); from then on every unit is level again.
+    const int dx_tiles = MODE == kBack ? p.dx_splits * m_tiles * p.n_tiles : 0;
+    const int dx_left = dx_tiles % units;
+    const int dx_mine = dx_tiles / units + (unit < dx_left ? 1 : 0);
+    const int dw_kbs = (rows + kBK - 1) / kBK;
+    const int dw_extra = dx_left > 0 ? (p.dx_kb_per + 6) / (dw_kbs + 6) : 0;
+    auto tile_at = [&](int i, Tile &tile) {
+        tile.split = 0;
+        tile.dw = false;
+        if (MODE != kBack) {
+            const int t = unit + i * units;
+            if (t >= m_tiles * p.n_tiles)
+                return false;
+            tile.m0 = (t % m_tiles) * C::kTileM + static_cast<int>(rank) * kBM;
+            tile.n0 = (t / m_tiles) * p.bn;
+            tile.kb0 = 0;
+            tile.kbn = p.num_kb;
+            return true;
+        }
+        // Columns fastest: the units at work share panels of G.
+        if (i < dx_mine) {
+            const int t = unit + i * units;
+            const int per_split = m_tiles * p.n_tiles;
+            tile.split = t / per_split;
+            const int r = t - tile.split * per_split;
+            tile.m0 = (r / p.n_tiles) * C::kTileM + static_cast<int>(rank) * kBM;
+            tile.n0 = (r % p.n_tiles) * p.bn;
+            tile.kb0 = tile.split * p.dx_kb_per;
+            tile.kbn = min(p.dx_kb_per, (p.vocab + kBK - 1) / kBK - tile.kb0);
+            return true;
+        }
+        const int j = i - dx_mine;
+        const bool early = unit >= dx_left;
+        const int t = early && j < dw_extra
+                          ? j * (units - dx_left) + unit - dx_left
+                          : (units - dx_left) * dw_extra + (j - (early ? dw_extra : 0)) * units + unit;
+        if (t >= p.dw_tiles)
+            return false;
+        tile.dw = true;
+        tile.m0 = (t / p.n_tiles) * C::kTileM + static_cast<int>(rank) * kBM;
+        tile.n0 = (t % p.n_tiles) * p.bn;
+        tile.kb0 = 0;
+        tile.kbn = dw_kbs;
+        return true;
+    };
+
     if (warp == 0) {
         // ---------------- TMA producer (one thread) ----------------
         if (lane == 0) {
@@ -322,11 +376,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             const int b_rows = kPair ? p.bn / 2 : p.bn; // this CTA's
             const int b_boxes = (b_rows + 63) / 64;     // MN-major
-            const uint32_t tx = (kPair ? 2u : 1u) * (static_cast<uint32_t>(C::kAMn ? kBM : p.a_rows) * 128u +
-                                                     (C::kBMn ? b_boxes * 8192u : b_rows * 128u));
-            for (int t = tile_first; ok && t < p.num_tiles; t += tile_step) {
-                const Tile tile = tile_at(t);
+            Tile tile;
+            for (int n = 0; ok && tile_at(n, tile); ++n) {
                 const int b0 = tile.n0 + static_cast<int>(rank) * b_rows;
+                const uint32_t tx = (kPair ? 2u : 1u) * (static_cast<uint32_t>(tile.dw ? kBM : p.a_rows) * 128u +
+                                                         (MODE == kBack ? b_boxes * 8192u : b_rows * 128u));
+                const CUtensorMap *map_b = tile.dw ? &tm_b2 : &tm_b;
                 for (int i = 0; i < tile.kbn; ++i) {
                     if (!mbar_wait(bar_empty + 8 * s, ph ^ 1u, kSiteProducerEmpty)) {
                         ok = false;
@@ -338,16 +393,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t full = kPair ? map_to_rank(bar_full + 8 * s, 0) : bar_full + 8 * s;
                     const uint32_t a = sbase + s * C::kABytes;
                     const uint32_t b = sbase + C::kOffB + s * C::kBBytes;
-                    if (C::kAMn) {
+                    if (MODE == kBack && tile.dw) {
 #pragma unroll
                         for (int j = 0; j < kBM / 64; ++j)
-                            load(a + j * 8192, &tm_a, full, tile.m0 + 64 * j, k0);
+                            load(a + j * 8192, &tm_a2, full, tile.m0 + 64 * j, k0);
                     } else {
                         load(a, &tm_a, full, k0, tile.m0);
                     }
-                    if (C::kBMn) {
+                    if (MODE == kBack) {
                         for (int j = 0; j < b_boxes; ++j)
-                            load(b + j * 8192, &tm_b, full, b0 + 64 * j, k0);
+                            load(b + j * 8192, map_b, full, b0 + 64 * j, k0);
                     } else {
                         load(b, &tm_b, full, k0, b0);
                     }
@@ -372,18 +427,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
         // ---------------- MMA issuer (one thread of the leader) ----------------
         if (lane == 0 && leader) {
-            const uint32_t idesc = C::kIdesc | p.idesc_bits;
             int s = 0;
             uint32_t ph = 0;
-            int local = 0;
             bool ok = true;
-            for (int t = tile_first; ok && t < p.num_tiles; t += tile_step) {
-                const Tile tile = tile_at(t);
-                if (tile.kbn <= 0)
-                    continue;
-                const uint32_t a = local & 1;
-                const uint32_t acc_ph = (local >> 1) & 1;
-                ++local;
+            Tile tile;
+            for (int n = 0; ok && tile_at(n, tile); ++n) {
+                const bool a_mn = MODE == kBack && tile.dw;
+                const uint32_t idesc =
+                    C::kIdesc | p.idesc_bits | (a_mn ? kAMnMajor : 0u) | (MODE == kBack ? kBMnMajor : 0u);
+                const uint32_t a = n & 1;
+                const uint32_t acc_ph = (n >> 1) & 1;
                 if (!mbar_wait(bar_acc_empty + 8 * a, acc_ph ^ 1u, kSiteMmaAccEmpty)) {
                     ok = false;
                     break;
@@ -401,10 +454,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int k = 0; k < kBK / kUmmaK; ++k) {
                         // 16 K elements: 32 bytes of a K-major row, or two 8-row atoms.
-                        const uint64_t da =
-                            C::kAMn ? desc_mn_boxes(a_addr + k * 2048) : smem_desc_k_sw128(a_addr + k * 32);
+                        const uint64_t da = a_mn ? desc_mn_boxes(a_addr + k * 2048) : smem_desc_k_sw128(a_addr + k * 32);
                         const uint64_t db =
-                            C::kBMn ? desc_mn_boxes(b_addr + k * 2048) : smem_desc_k_sw128(b_addr + k * 32);
+                            MODE == kBack ? desc_mn_boxes(b_addr + k * 2048) : smem_desc_k_sw128(b_addr + k * 32);
                         if (kPair)
                             mma_f16_pair(d_tmem, da, db, idesc, (i | k) != 0);
                         else
@@ -435,39 +487,55 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else {
-        // ---------------- Epilogue: 16 warps, one row per lane ----------------
+        // ---------------- Epilogue: one row per lane ----------------
         const int ew = warp - 2;
         const int quarter = warp & 3;
-        // This warp's columns: of the tile's 32-column steps, about a quarter.
+        // This warp's columns: its share of the tile's 32-column steps.
         const int slice = ew >> 2;
         const int steps = (p.bn + kSub - 1) / kSub;
-        const int col_begin = slice * steps / 4 * kSub;
-        const int col_end = min((slice + 1) * steps / 4 * kSub, p.bn);
+        const int col_begin = slice * steps / C::kParts * kSub;
+        const int col_end = min((slice + 1) * steps / C::kParts * kSub, p.bn);
         const uint32_t acc_empty = kPair ? map_to_rank(bar_acc_empty, 0) : bar_acc_empty;
         uint8_t *staging = smem + C::kOffStaging + ew * C::kStaging;
         const uint32_t staging_s = smem_u32(staging);
-        const float inv_gain = MODE == kDw || (MODE == kDx && !kPlanes) ? *p.inv_gain : 1.0f;
-        int local = 0;
-        for (int t = tile_first; t < p.num_tiles; t += tile_step) {
-            const Tile tile = tile_at(t);
-            if (tile.kbn <= 0)
-                continue;
-            const uint32_t a = local & 1;
-            const uint32_t acc_ph = (local >> 1) & 1;
-            ++local;
+        const float inv_gain = MODE == kBack ? *p.inv_gain : 1.0f;
+        uint32_t stores = 0;
+        // A staging buffer (32 rows x 64 B, 64-byte swizzle: chunk j of row r at j ^ ((r >> 1) & 3))
+        // that its last store has read, its filling, and the fence before the next store.
+        auto next_buffer = [&] {
+            if (lane == 0)
+                asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(C::kBuffers - 1) : "memory");
+            __syncwarp();
+            return C::kBuffers > 1 ? (stores++ & 1u) * 2048u : 0u;
+        };
+        auto put = [&](uint32_t buffer, int j, uint4 w) {
+            *reinterpret_cast<uint4 *>(staging + buffer + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) = w;
+        };
+        auto filled = [&] {
+            fence_proxy_async_smem();
+            __syncwarp();
+        };
+        Tile tile;
+        for (int n = 0; tile_at(n, tile); ++n) {
+            const uint32_t a = n & 1;
+            const uint32_t acc_ph = (n >> 1) & 1;
+            // G is also written (as zeros) for the rows that fill up a K block of dW.
+            const int row_limit = MODE == kBack && tile.dw ? p.vocab
+                                  : MODE == kGrad          ? min((rows + kBK - 1) / kBK * kBK, p.rows)
+                                                           : rows;
             const int row0 = tile.m0 + quarter * 32;
             const int row = row0 + lane;
             const int col0 = tile.n0 + col_begin;
             const int col1 = min(tile.n0 + col_end, p.n);
             // Rows and columns of this warp that exist.
-            const int width = row0 < p.m ? col1 - col0 : 0;
+            const int width = row0 < row_limit ? col1 - col0 : 0;
             int subs = width > 0 ? (width + kSub - 1) / kSub : 0;
 
             // The row's next target column (relative to the piece), found while the MMAs run.
             int next = INT_MAX, entry = 0;
             const int32_t *row_cols = nullptr;
             float lse2 = 0.0f, gain = 0.0f;
-            if ((MODE == kStats || MODE == kGrad) && row < p.m && subs > 0) {
+            if (MODE != kBack && row < rows && subs > 0) {
                 if (p.t_index) {
                     row_cols = p.t_index + static_cast<size_t>(row) * p.targets;
                     entry = lower_bound(row_cols, p.targets, p.col0 + col0);
@@ -576,47 +644,46 @@ __global__ void __launch_bounds__(kThreads, 1)
                             next = entry < p.targets ? row_cols[entry] - p.col0 : INT_MAX;
                         }
                     }
-                } else {
+                }
+                if (MODE == kBack && !tile.dw) {
+                    // fp32, 16 columns at a time.
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const uint32_t buffer = next_buffer();
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            put(buffer, j,
+                                make_uint4(v[16 * hf + 4 * j], v[16 * hf + 4 * j + 1], v[16 * hf + 4 * j + 2],
+                                           v[16 * hf + 4 * j + 3]));
+                        filled();
+                        if (lane == 0) {
+                            if (c0 + 16 * hf < p.n) {
+                                if (p.accumulate)
+                                    tma_store_add_3d(&tm_out, staging_s + buffer, c0 + 16 * hf, row0, tile.split);
+                                else
+                                    tma_store_3d(&tm_out, staging_s + buffer, c0 + 16 * hf, row0, tile.split);
+                            }
+                            bulk_commit_group();
+                        }
+                    }
+                    continue;
+                }
+                if (MODE == kBack) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         f[i] = __uint_as_float(v[i]) * inv_gain;
                 }
-                // Staging: 32 rows x 64 B, 64-byte swizzle: chunk j of row r at j ^ ((r >> 1) & 3).
-                constexpr int kSteps = MODE == kDx && kPlanes ? 2 : 1; // fp32: 16 columns at a time
+                const uint32_t buffer = next_buffer();
 #pragma unroll
-                for (int hf = 0; hf < kSteps; ++hf) {
-                    if (lane == 0)
-                        bulk_wait_group_read0(); // the previous store has read the buffer
-                    __syncwarp();
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint4 w;
-                        if (kSteps == 2) {
-                            w = make_uint4(__float_as_uint(f[16 * hf + 4 * j]), __float_as_uint(f[16 * hf + 4 * j + 1]),
-                                           __float_as_uint(f[16 * hf + 4 * j + 2]),
-                                           __float_as_uint(f[16 * hf + 4 * j + 3]));
-                        } else {
-                            w = make_uint4(pack16(f[8 * j], f[8 * j + 1], kBf16), pack16(f[8 * j + 2], f[8 * j + 3], kBf16),
-                                           pack16(f[8 * j + 4], f[8 * j + 5], kBf16),
-                                           pack16(f[8 * j + 6], f[8 * j + 7], kBf16));
-                        }
-                        *reinterpret_cast<uint4 *>(staging + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) = w;
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (kSteps == 2) {
-                            if (c0 + 16 * hf < p.n) {
-                                if (p.accumulate)
-                                    tma_store_add_3d(&tm_out, staging_s, c0 + 16 * hf, row0, tile.split);
-                                else
-                                    tma_store_3d(&tm_out, staging_s, c0 + 16 * hf, row0, tile.split);
-                            }
-                        } else {
-                            tma_store_2d(&tm_out, staging_s, c0, row0);
-                        }
-                        bulk_commit_group();
-                    }
+                for (int j = 0; j < 4; ++j)
+                    put(buffer, j,
+                        make_uint4(pack16(f[8 * j], f[8 * j + 1], kBf16), pack16(f[8 * j + 2], f[8 * j + 3], kBf16),
+                                   pack16(f[8 * j + 4], f[8 * j + 5], kBf16),
+                                   pack16(f[8 * j + 6], f[8 * j + 7], kBf16)));
+                filled();
+                if (lane == 0) {
+                    tma_store_2d(MODE == kBack ? &tm_out2 : &tm_out, staging_s + buffer, c0, row0);
+                    bulk_commit_group();
                 }
             }
             if (subs == 0) {
@@ -630,16 +697,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if (MODE == kStats) {
-                // Merge the four column slices of each row: the warps of a quarter meet on a
+                // Merge the column slices of each row: the warps of a quarter meet on a
                 // named barrier, and the first writes the tile's partial result.
-                float *mine = reinterpret_cast<float *>(staging) + (local & 1) * 96;
+                float *mine = reinterpret_cast<float *>(staging) + (n & 1) * 96;
                 mine[lane] = run_max;
                 mine[32 + lane] = run_sum;
                 mine[64 + lane] = run_t;
-                named_barrier_sync(1 + quarter, 128);
-                if (slice == 0 && row < p.m) {
+                named_barrier_sync(1 + quarter, 32 * C::kParts);
+                if (slice == 0 && row < rows) {
 #pragma unroll
-                    for (int j = 1; j < 4; ++j) {
+                    for (int j = 1; j < C::kParts; ++j) {
                         const float *other = mine + j * (4 * C::kStaging / 4);
                         const float m = other[lane];
                         const float next_max = fmaxf(run_max, m);
@@ -648,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         run_max = next_max;
                         run_t += other[64 + lane];
                     }
-                    const size_t at = static_cast<size_t>(tile.n0 / p.bn) * p.m + row;
+                    const size_t at = static_cast<size_t>(tile.n0 / p.bn) * rows + row;
                     p.part_max[at] = run_max;
                     p.part_sum[at] = run_sum;
                     if (p.part_t)
@@ -828,20 +895,131 @@ struct Prepare {
     float temperature;
     int width;            // elements per row of x, a multiple of 8
     const void *x;
-    void *x_masked;
+    void *x_used;
     const float *lse, *grad;
     float *row_lse2, *row_gain, *inv_gain;
+    int *rows_used, *row_at; // labels: how many rows have a target, and where each went (-1: nowhere)
 };
 
-// Backward's first step: per row its targets, lse and gain g T s, and a copy of x whose rows
-// without a target are zero, so that whatever those hold (NaN included) reaches neither G nor
-// dW.  s = 2^(13 - exponent of max |g T|) puts |g T s| in [2^13, 2^14): with |p - t| <= 1, G
-// then fits fp16 and keeps 11 bits down to p = 2^-28.
-// R = 0: one label per row; otherwise up to 32 R teacher entries.
-template <int R>
-__global__ void __launch_bounds__(32 * kPrepWarps) prepare_kernel(const Prepare p)
+// s = 2^(13 - exponent of max |g T|) puts |g T s| in [2^13, 2^14): with |p - t| <= 1, G then
+// fits fp16 and keeps 11 bits down to p = 2^-28.  Returns s; thread 0 of block 0 keeps 1 / s.
+__device__ __forceinline__ float common_gain(float top, float *inv_gain)
 {
-    __shared__ float probs[kPrepWarps][R > 0 ? 32 * R : 1];
+    const int exponent = top > 0.0f && top < INFINITY ? min(max(ilogbf(top), -100), 100) : 13;
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        *inv_gain = ldexpf(1.0f, exponent - 13);
+    return ldexpf(1.0f, 13 - exponent);
+}
+
+constexpr int kHeadVectors = 5; // 1280 elements of a row per lane group, requested ahead
+
+// Backward's first step with labels.  The rows that have a target move together, in order:
+// their states, labels, lse and gain g T s.  The others (padding, in a batch of transcripts)
+// take no part in the products, so whatever they hold, NaN included, reaches nothing and costs
+// nothing.  Up to 255 zero rows follow, to the end of a tile, so that what a tile reads there
+// adds nothing.  Each block counts the valid labels before its rows itself (a few KB of reads).
+__global__ void __launch_bounds__(32 * kPrepWarps) prepare_rows_kernel(const Prepare p, int rows_per_block)
+{
+    __shared__ float warp_max[kPrepWarps];
+    __shared__ int warp_before[kPrepWarps], warp_total[kPrepWarps];
+    griddepcontrol_wait();
+    griddepcontrol_launch_dependents();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int begin = min(static_cast<int>(blockIdx.x) * rows_per_block, p.t.rows);
+    const int end = min(begin + rows_per_block, p.t.rows);
+    auto valid = [&](int64_t label) { return label != p.ignore_index && label >= 0 && label < p.t.vocab; };
+    float top = 0.0f;
+    int before = 0, total = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < p.t.rows; i += 32 * kPrepWarps) {
+        const float g = fabsf(__ldg(p.grad + i));
+        const bool used = valid(load_label(p.labels, p.label_bytes, i));
+        top = fmaxf(top, used && g < INFINITY ? g : 0.0f);
+        before += used && i < begin;
+        total += used;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    if (lane == 0) {
+        warp_max[warp] = top;
+        warp_before[warp] = before;
+        warp_total[warp] = total;
+    }
+    __syncthreads();
+    top = 0.0f;
+    before = total = 0;
+#pragma unroll
+    for (int i = 0; i < kPrepWarps; ++i) {
+        top = fmaxf(top, warp_max[i]);
+        before += warp_before[i];
+        total += warp_total[i];
+    }
+    const float s = common_gain(top * p.temperature, p.inv_gain);
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        *p.rows_used = max(total, 1); // a row of zeros where no row has a target
+
+    const int vectors = p.width / 8;
+    const uint4 *x = static_cast<const uint4 *>(p.x);
+    uint4 *x_used = static_cast<uint4 *>(p.x_used);
+    for (int first = begin; first < end; first += 32) {
+        const int64_t mine = first + lane < end ? load_label(p.labels, p.label_bytes, first + lane) : p.ignore_index;
+        const uint32_t mask = __ballot_sync(0xffffffffu, valid(mine));
+        if (warp == 0 && first + lane < end) {
+            if (!valid(mine) && mine != p.ignore_index)
+                g_token_error = 1;
+            p.row_at[first + lane] = valid(mine) ? before + __popc(mask & ((1u << lane) - 1u)) : -1;
+        }
+        for (int j = warp; j < 32; j += kPrepWarps) {
+            if (!(mask >> j & 1u))
+                continue;
+            const int row = first + j, to = before + __popc(mask & ((1u << j) - 1u));
+            const uint4 *src = x + static_cast<size_t>(row) * vectors;
+            uint4 *dst = x_used + static_cast<size_t>(to) * vectors;
+            uint4 head[kHeadVectors];
+#pragma unroll
+            for (int i = 0; i < kHeadVectors; ++i)
+                if (lane + 32 * i < vectors)
+                    head[i] = __ldg(src + lane + 32 * i);
+#pragma unroll
+            for (int i = 0; i < kHeadVectors; ++i)
+                if (lane + 32 * i < vectors)
+                    dst[lane + 32 * i] = head[i];
+            for (int i = lane + 32 * kHeadVectors; i < vectors; i += 32)
+                dst[i] = __ldg(src + i);
+            const int64_t label = __shfl_sync(0xffffffffu, mine, j);
+            if (lane == 0) {
+                p.t.index[to] = static_cast<int32_t>(label);
+                p.t.prob[to] = 1.0f;
+                p.row_lse2[to] = p.lse[row] * kLog2e;
+                p.row_gain[to] = p.grad[row] * p.temperature * s;
+            }
+        }
+        before += __popc(mask);
+    }
+    const int tail = min(max((total + 255) / 256, 1) * 256, p.t.rows);
+    for (int row = total + blockIdx.x * kPrepWarps + warp; row < tail; row += gridDim.x * kPrepWarps) {
+        for (int i = lane; i < vectors; i += 32)
+            x_used[static_cast<size_t>(row) * vectors + i] = make_uint4(0u, 0u, 0u, 0u);
+        if (lane == 0) {
+            p.t.index[row] = INT_MAX;
+            p.t.prob[row] = 0.0f;
+            p.row_lse2[row] = 0.0f;
+            p.row_gain[row] = 0.0f;
+        }
+    }
+}
+
+// Backward's first step with a teacher: per row its sorted targets (up to 32 R), lse and gain,
+// and a copy of x whose rows without a target are zero, so that whatever those hold, NaN
+// included, reaches neither G nor dW.
+template <int R>
+__global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const Prepare p)
+{
+    __shared__ float probs[kPrepWarps][32 * R];
     __shared__ float warp_max[kPrepWarps];
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
@@ -863,46 +1041,30 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_kernel(const Prepare 
 #pragma unroll
     for (int i = 0; i < kPrepWarps; ++i)
         top = fmaxf(top, warp_max[i]);
-    top *= p.temperature;
-    const int exponent = top > 0.0f && top < INFINITY ? min(max(ilogbf(top), -100), 100) : 13;
-    const float s = ldexpf(1.0f, 13 - exponent);
-    if (blockIdx.x == 0 && threadIdx.x == 0)
-        *p.inv_gain = ldexpf(1.0f, exponent - 13);
+    const float s = common_gain(top * p.temperature, p.inv_gain);
 
+    const int vectors = p.width / 8;
     for (int row = blockIdx.x * kPrepWarps + warp; row < p.t.rows; row += gridDim.x * kPrepWarps) {
-        const int vectors = p.width / 8;
         const size_t base = static_cast<size_t>(row) * vectors;
         const uint4 *src = static_cast<const uint4 *>(p.x) + base;
-        uint4 *dst = static_cast<uint4 *>(p.x_masked) + base;
-        // The row's first 1280 elements are requested before its targets are known.
-        uint4 head[5];
+        uint4 *dst = static_cast<uint4 *>(p.x_used) + base;
+        // The start of the row is requested before its targets are known.
+        uint4 head[kHeadVectors];
 #pragma unroll
-        for (int i = 0; i < 5; ++i)
+        for (int i = 0; i < kHeadVectors; ++i)
             if (lane + 32 * i < vectors)
                 head[i] = __ldg(src + lane + 32 * i);
-        bool any;
-        if constexpr (R > 0) {
-            double entropy, total;
-            any = sort_targets<R>(p.t, row, lane, probs[warp], entropy, total);
-        } else {
-            const int64_t label = load_label(p.labels, p.label_bytes, row);
-            any = label != p.ignore_index && label >= 0 && label < p.t.vocab;
-            if (lane == 0) {
-                if (!any && label != p.ignore_index)
-                    g_token_error = 1;
-                p.t.index[row] = any ? static_cast<int32_t>(label) : INT_MAX;
-                p.t.prob[row] = 1.0f;
-            }
-        }
+        double entropy, total;
+        const bool any = sort_targets<R>(p.t, row, lane, probs[warp], entropy, total);
         if (lane == 0) {
             p.row_lse2[row] = any ? p.lse[row] * kLog2e : 0.0f;
             p.row_gain[row] = any ? p.grad[row] * p.temperature * s : 0.0f;
         }
 #pragma unroll
-        for (int i = 0; i < 5; ++i)
+        for (int i = 0; i < kHeadVectors; ++i)
             if (lane + 32 * i < vectors)
                 dst[lane + 32 * i] = any ? head[i] : make_uint4(0u, 0u, 0u, 0u);
-        for (int i = lane + 160; i < vectors; i += 32)
+        for (int i = lane + 32 * kHeadVectors; i < vectors; i += 32)
             dst[i] = any ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
     }
 }
@@ -1096,25 +1258,45 @@ __global__ void __launch_bounds__(32 * kCombineRowWarps) combine_rows_kernel(con
         write_row(p, row, mx, sum, target, label_z);
 }
 
-// dx = sum of the fp32 planes (one per K split), in order, times 1 / s: eight elements per thread.
+// dx = sum of the fp32 planes (one per K split), in order, times 1 / s; rows that moved come
+// from where they went, rows without a target are zero.  Eight elements per thread, the loads
+// of eight planes in flight; blocks own rows (blockIdx.x, then a grid's stride on).
 template <bool kBf16>
-__global__ void __launch_bounds__(256) planes_kernel(const float *planes, int count, size_t elements,
-                                                     const float *inv_gain, uint4 *dx)
+__global__ void __launch_bounds__(256) planes_kernel(const float *planes, int count, int rows, int width,
+                                                     const int *row_at, const float *inv_gain, uint4 *dx)
 {
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
     const float inv = *inv_gain;
-    for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < elements / 8;
-         i += static_cast<size_t>(gridDim.x) * blockDim.x) {
-        float f[8] = {};
-        for (int s = 0; s < count; ++s) {
-            const float4 *src = reinterpret_cast<const float4 *>(planes + s * elements) + 2 * i;
-            const float4 lo = src[0], hi = src[1];
-            f[0] += lo.x, f[1] += lo.y, f[2] += lo.z, f[3] += lo.w;
-            f[4] += hi.x, f[5] += hi.y, f[6] += hi.z, f[7] += hi.w;
-        }
-        dx[i] = make_uint4(pack16(f[0] * inv, f[1] * inv, kBf16), pack16(f[2] * inv, f[3] * inv, kBf16),
+    const int vectors = width / 8;
+    const size_t plane = static_cast<size_t>(rows) * vectors; // in pairs of float4
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+        const int from = row_at ? __ldg(row_at + row) : row;
+        for (int i = threadIdx.x; i < vectors; i += blockDim.x) {
+            float f[8] = {};
+            if (from >= 0) {
+                const float4 *src =
+                    reinterpret_cast<const float4 *>(planes) + 2 * (static_cast<size_t>(from) * vectors + i);
+                for (int s = 0; s < count; s += 8) {
+                    float4 lo[8], hi[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (s + j < count) {
+                            lo[j] = __ldg(src + 2 * plane * (s + j));
+                            hi[j] = __ldg(src + 2 * plane * (s + j) + 1);
+                        }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (s + j < count) {
+                            f[0] += lo[j].x, f[1] += lo[j].y, f[2] += lo[j].z, f[3] += lo[j].w;
+                            f[4] += hi[j].x, f[5] += hi[j].y, f[6] += hi[j].z, f[7] += hi[j].w;
+                        }
+                }
+            }
+            dx[static_cast<size_t>(row) * vectors + i] =
+                make_uint4(pack16(f[0] * inv, f[1] * inv, kBf16), pack16(f[2] * inv, f[3] * inv, kBf16),
                            pack16(f[4] * inv, f[5] * inv, kBf16), pack16(f[6] * inv, f[7] * inv, kBf16));
+        }
     }
 }
 
@@ -1226,28 +1408,30 @@ ForwardPlan plan_forward(const VocabLossLaunch &L, void *workspace)
 }
 
 struct BackwardPlan {
-    bool single;
+    bool single;             // kGrad by one CTA per tile
     int targets;
     int64_t piece, pieces;   // vocabulary columns per piece of G
     int64_t ldg;             // elements per row of a piece
     int grad_bn, width_bn;   // tile widths over a piece's columns, and over x's width
     int64_t splits;          // K splits of dx
-    bool planes;
     float *row_lse2, *row_gain, *inv_gain, *t_prob, *dx_planes;
     int32_t *t_index;
-    void *x_masked, *g;
+    int *rows_used, *row_at;
+    void *x_used, *g;
     int64_t bytes;
 };
 
 // K splits of dx = G W, whose tiles (rows x width) are few while its K axis, a piece of the
-// vocabulary, is long.  The splits that finish first by a count of K blocks: rounds of the
-// persistent CTAs times a tile's blocks (and about four for its start and epilogue), plus the
-// fp32 planes' write and read at 1.6 MB per block's time (0.33 us at 5 TB/s).  3584 x 768 x
-// 51865: 42 tiles for 74 pairs, one split 265 us, three splits 190 us with their planes.
+// vocabulary, is long: the count that finishes first, by K blocks of a CTA pair.  dx and dW
+// tiles share one launch, so its time is the mean over the pairs or the rounds of dx tiles
+// alone, whichever is longer (about six blocks for a tile's start and epilogue), plus the fp32
+// planes' write and read at 1.6 MB per block's time (0.33 us at 5 TB/s).
 int64_t dx_splits(const VocabLossLaunch &L, const BackwardPlan &b)
 {
-    const int64_t units = b.single ? sm_count() : sm_count() / 2;
-    const int64_t tiles = ceil_div(L.rows, b.single ? kBM : 2 * kBM) * ceil_div(L.width, b.width_bn);
+    const int64_t units = sm_count() / 2;
+    const int64_t n_tiles = ceil_div(L.width, b.width_bn);
+    const int64_t dx_tiles = ceil_div(L.rows, 2 * kBM) * n_tiles;
+    const int64_t dw = L.dweight ? ceil_div(b.piece, 2 * kBM) * n_tiles * (ceil_div(L.rows, kBK) + 6) : 0;
     const int64_t kbs = ceil_div(b.piece, kBK);
     int64_t best = 1;
     double best_cost = INFINITY;
@@ -1256,9 +1440,9 @@ int64_t dx_splits(const VocabLossLaunch &L, const BackwardPlan &b)
         if (s > 1 && per < 4)
             break;
         const int64_t used = ceil_div(kbs, per);
-        const bool planes = used > 1 || b.pieces > 1;
-        const double cost = static_cast<double>(ceil_div(tiles * used, units) * (per + 4)) * b.pieces +
-                            (planes ? static_cast<double>(used) * L.rows * L.width * 8 / 1.6e6 : 0.0);
+        const double mean = static_cast<double>(dx_tiles * used * (per + 6) + dw) / units;
+        const double rounds = static_cast<double>(ceil_div(dx_tiles * used, units) * (per + 6));
+        const double cost = std::max(mean, rounds) * b.pieces + static_cast<double>(used) * L.rows * L.width * 8 / 1.6e6;
         if (cost < best_cost) {
             best_cost = cost;
             best = used;
@@ -1280,17 +1464,19 @@ BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
     b.ldg = round_up(b.piece, 64);
     b.grad_bn = logits_width(L.rows, b.piece, L.width, b.single, 32);
     b.width_bn = even_width(L.width);
-    b.splits = dx_splits(L, b);
-    b.planes = b.splits > 1 || b.pieces > 1;
+    b.splits = L.dx ? dx_splits(L, b) : 0;
     b.row_lse2 = arena.take<float>(L.rows);
     b.row_gain = arena.take<float>(L.rows);
     b.inv_gain = arena.take<float>(1);
     b.t_index = arena.take<int32_t>(L.rows * b.targets);
     b.t_prob = arena.take<float>(L.rows * b.targets);
-    b.x_masked = arena.take<uint16_t>(L.rows * L.width);
+    if (L.targets == 0) {
+        b.rows_used = arena.take<int>(1);
+        b.row_at = arena.take<int>(L.rows);
+    }
+    b.x_used = arena.take<uint16_t>(L.rows * L.width);
     b.g = arena.take<uint16_t>(L.rows * b.ldg);
-    if (L.dx && b.planes)
-        b.dx_planes = arena.take<float>(b.splits * L.rows * L.width);
+    b.dx_planes = arena.take<float>(b.splits * L.rows * L.width);
     b.bytes = arena.used;
     return b;
 }
@@ -1316,13 +1502,12 @@ bool operand_map(CUtensorMap *map, bool bf16, bool mn_major, const void *base, i
                     : map16(map, bf16, base, rows, cols, ld, kBK, mn_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// p: m, n, bn and num_kb, kb_per set.
-template <bool kPair, int MODE, bool kBf16, bool kPlanes>
-cudaError_t launch_one(const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &out, Params p,
-                       cudaStream_t stream)
+// maps: A, B, output, and kBack's second A, B, output.  `tiles`: the most there can be.
+template <bool kPair, int MODE, bool kBf16>
+cudaError_t launch_one(const CUtensorMap (&maps)[6], int64_t tiles, Params p, cudaStream_t stream)
 {
     using C = Cfg<kPair, MODE>;
-    auto kernel = gemm_kernel<kPair, MODE, kBf16, kPlanes>;
+    auto kernel = gemm_kernel<kPair, MODE, kBf16>;
     static std::atomic<bool> opted[kMaxDevices];
     const int device = current_device();
     if (!opted[device].load(std::memory_order_acquire)) {
@@ -1332,16 +1517,12 @@ cudaError_t launch_one(const CUtensorMap &a, const CUtensorMap &b, const CUtenso
             return err;
         opted[device].store(true, std::memory_order_release);
     }
-    p.m_tiles = static_cast<int>(ceil_div(p.m, C::kTileM));
-    p.n_tiles = static_cast<int>(ceil_div(p.n, p.bn));
-    const int64_t splits = ceil_div(p.num_kb, p.kb_per);
-    p.num_tiles = static_cast<int>(splits * p.m_tiles * p.n_tiles);
-    p.a_rows = tile_rows(p.m);
+    p.a_rows = tile_rows(p.rows);
     p.idesc_bits = (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (static_cast<uint32_t>(p.bn >> 3) << 17);
-    const int units = kPair ? sm_count() / 2 : sm_count();
+    const int64_t units = kPair ? sm_count() / 2 : sm_count();
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(std::min(p.num_tiles, units) * (kPair ? 2 : 1)));
-    config.blockDim = dim3(kThreads);
+    config.gridDim = dim3(static_cast<unsigned>(std::min(tiles, units) * (kPair ? 2 : 1)));
+    config.blockDim = dim3(C::kThreads);
     config.dynamicSmemBytes = C::kSmemBytes;
     config.stream = stream;
     cudaLaunchAttribute attrs[2];
@@ -1356,7 +1537,7 @@ cudaError_t launch_one(const CUtensorMap &a, const CUtensorMap &b, const CUtenso
         config.numAttrs = 2;
     }
     config.attrs = attrs;
-    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, a, b, out, p);
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p);
     count_launch();
     return err != cudaSuccess ? err : cudaGetLastError();
 }
@@ -1364,21 +1545,25 @@ cudaError_t launch_one(const CUtensorMap &a, const CUtensorMap &b, const CUtenso
 // z tiles: x [rows, width] times columns [col0, col0 + cols) of W^T.
 template <int MODE, bool kBf16>
 cudaError_t launch_logits(const VocabLossLaunch &L, const void *x, int64_t col0, int64_t cols, int bn, bool single,
-                          const CUtensorMap &out, Params p, cudaStream_t stream)
+                          const CUtensorMap *out, Params p, cudaStream_t stream)
 {
-    CUtensorMap a, b;
+    CUtensorMap maps[6] = {};
     const uint16_t *w = static_cast<const uint16_t *>(L.weight) + col0 * L.width;
-    if (!operand_map(&a, kBf16, false, x, L.rows, L.width, L.width, tile_rows(L.rows)) ||
-        !operand_map(&b, kBf16, false, w, cols, L.width, L.width, single ? bn : bn / 2))
+    if (!operand_map(&maps[0], kBf16, false, x, L.rows, L.width, L.width, tile_rows(L.rows)) ||
+        !operand_map(&maps[1], kBf16, false, w, cols, L.width, L.width, single ? bn : bn / 2))
         return cudaErrorInvalidValue;
-    p.m = static_cast<int>(L.rows);
+    if (out)
+        maps[2] = *out;
+    p.rows = static_cast<int>(L.rows);
     p.n = static_cast<int>(cols);
     p.bn = bn;
+    p.n_tiles = static_cast<int>(ceil_div(cols, bn));
+    p.num_kb = static_cast<int>(ceil_div(L.width, kBK));
     p.col0 = static_cast<int>(col0);
-    p.num_kb = p.kb_per = static_cast<int>(ceil_div(L.width, kBK));
     p.scale2 = static_cast<float>(1.4426950408889634 / static_cast<double>(L.temperature));
-    return single ? launch_one<false, MODE, kBf16, false>(a, b, out, p, stream)
-                  : launch_one<true, MODE, kBf16, false>(a, b, out, p, stream);
+    const int64_t tiles = ceil_div(L.rows, single ? kBM : 2 * kBM) * p.n_tiles;
+    return single ? launch_one<false, MODE, kBf16>(maps, tiles, p, stream)
+                  : launch_one<true, MODE, kBf16>(maps, tiles, p, stream);
 }
 
 template <bool kBf16>
@@ -1415,7 +1600,7 @@ cudaError_t run_forward(const VocabLossLaunch &L, cudaStream_t stream)
     p.part_sum = f.part_sum;
     p.part_t = f.part_t;
     p.label_z = f.label_z;
-    err = launch_logits<kStats, kBf16>(L, L.x, 0, L.vocab, f.bn, f.single, CUtensorMap{}, p, stream);
+    err = launch_logits<kStats, kBf16>(L, L.x, 0, L.vocab, f.bn, f.single, nullptr, p, stream);
     if (err != cudaSuccess)
         return err;
     Combine c{};
@@ -1443,59 +1628,47 @@ cudaError_t run_forward(const VocabLossLaunch &L, cudaStream_t stream)
                       stream, c);
 }
 
+// dx (added up in the planes) and dW's rows from the piece of G over columns [col0, col0 + cols).
 template <bool kBf16>
-cudaError_t launch_dx(const VocabLossLaunch &L, const BackwardPlan &b, int64_t col0, int64_t cols, bool first,
-                      cudaStream_t stream)
+cudaError_t launch_back(const VocabLossLaunch &L, const BackwardPlan &b, int64_t col0, int64_t cols,
+                        cudaStream_t stream)
 {
-    CUtensorMap ma, mb, out;
-    const uint16_t *w = static_cast<const uint16_t *>(L.weight) + col0 * L.width;
-    if (!operand_map(&ma, kBf16, false, b.g, L.rows, cols, b.ldg, tile_rows(L.rows)) ||
-        !operand_map(&mb, kBf16, true, w, cols, L.width, L.width, 0))
-        return cudaErrorInvalidValue;
-    if (b.planes) {
+    CUtensorMap maps[6] = {};
+    Params p{};
+    p.rows = static_cast<int>(L.rows);
+    p.rows_used = b.rows_used;
+    p.n = static_cast<int>(L.width);
+    p.bn = b.width_bn;
+    p.n_tiles = static_cast<int>(ceil_div(L.width, b.width_bn));
+    p.vocab = static_cast<int>(cols);
+    p.inv_gain = b.inv_gain;
+    p.accumulate = col0 > 0 ? 1 : 0;
+    p.dx_kb_per = 1;
+    int64_t tiles = 0;
+    if (L.dx) {
+        const uint16_t *w = static_cast<const uint16_t *>(L.weight) + col0 * L.width;
         const int64_t dims[3] = {L.width, L.rows, b.splits};
         const int64_t strides[2] = {L.width * 4, L.rows * L.width * 4};
         const uint32_t box[3] = {16u, 32u, 1u};
-        if (!make_map_nd(&out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, b.dx_planes, dims, strides, box,
+        if (!operand_map(&maps[0], kBf16, false, b.g, L.rows, cols, b.ldg, tile_rows(L.rows)) ||
+            !operand_map(&maps[1], kBf16, true, w, cols, L.width, L.width, 0) ||
+            !make_map_nd(&maps[2], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, b.dx_planes, dims, strides, box,
                          CU_TENSOR_MAP_SWIZZLE_64B))
             return cudaErrorInvalidValue;
-    } else if (!map16(&out, kBf16, L.dx, L.rows, L.width, L.width, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
-        return cudaErrorInvalidValue;
+        p.dx_kb_per = static_cast<int>(ceil_div(ceil_div(b.piece, kBK), b.splits));
+        p.dx_splits = static_cast<int>(ceil_div(ceil_div(cols, kBK), p.dx_kb_per)); // a last piece has fewer
+        tiles += p.dx_splits * ceil_div(L.rows, 2 * kBM) * p.n_tiles;
     }
-    Params p{};
-    p.m = static_cast<int>(L.rows);
-    p.n = static_cast<int>(L.width);
-    p.num_kb = static_cast<int>(ceil_div(cols, kBK));
-    p.kb_per = static_cast<int>(ceil_div(ceil_div(b.piece, kBK), b.splits));
-    p.bn = b.width_bn;
-    p.n_first = 1;
-    p.inv_gain = b.inv_gain;
-    p.accumulate = first ? 0 : 1;
-    if (b.planes)
-        return b.single ? launch_one<false, kDx, kBf16, true>(ma, mb, out, p, stream)
-                        : launch_one<true, kDx, kBf16, true>(ma, mb, out, p, stream);
-    return b.single ? launch_one<false, kDx, kBf16, false>(ma, mb, out, p, stream)
-                    : launch_one<true, kDx, kBf16, false>(ma, mb, out, p, stream);
-}
-
-template <bool kBf16>
-cudaError_t launch_dw(const VocabLossLaunch &L, const BackwardPlan &b, int64_t col0, int64_t cols,
-                      cudaStream_t stream)
-{
-    CUtensorMap ma, mb, out;
-    uint16_t *dw = static_cast<uint16_t *>(L.dweight) + col0 * L.width;
-    if (!operand_map(&ma, kBf16, true, b.g, L.rows, cols, b.ldg, 0) ||
-        !operand_map(&mb, kBf16, true, b.x_masked, L.rows, L.width, L.width, 0) ||
-        !map16(&out, kBf16, dw, cols, L.width, L.width, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B))
-        return cudaErrorInvalidValue;
-    Params p{};
-    p.m = static_cast<int>(cols);
-    p.n = static_cast<int>(L.width);
-    p.num_kb = p.kb_per = static_cast<int>(ceil_div(L.rows, kBK));
-    p.bn = b.width_bn;
-    p.n_first = 1;
-    p.inv_gain = b.inv_gain;
-    return launch_one<true, kDw, kBf16, false>(ma, mb, out, p, stream);
+    if (L.dweight) {
+        uint16_t *dw = static_cast<uint16_t *>(L.dweight) + col0 * L.width;
+        if (!operand_map(&maps[3], kBf16, true, b.g, L.rows, cols, b.ldg, 0) ||
+            !operand_map(&maps[4], kBf16, true, b.x_used, L.rows, L.width, L.width, 0) ||
+            !map16(&maps[5], kBf16, dw, cols, L.width, L.width, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B))
+            return cudaErrorInvalidValue;
+        p.dw_tiles = static_cast<int>(ceil_div(cols, 2 * kBM) * p.n_tiles);
+        tiles += p.dw_tiles;
+    }
+    return launch_one<true, kBack, kBf16>(maps, tiles, p, stream);
 }
 
 template <bool kBf16>
@@ -1518,20 +1691,26 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
     q.temperature = L.temperature;
     q.width = static_cast<int>(L.width);
     q.x = L.x;
-    q.x_masked = b.x_masked;
+    q.x_used = b.x_used;
     q.lse = L.lse_in;
     q.grad = L.dloss;
     q.row_lse2 = b.row_lse2;
     q.row_gain = b.row_gain;
     q.inv_gain = b.inv_gain;
-    const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, kPrepWarps), 4 * sm_count());
-    const dim3 grid(static_cast<unsigned>(blocks)), block(32 * kPrepWarps);
-    cudaError_t err = L.targets > 0 ? per_lane(L.targets,
-                                               [&](auto r) {
-                                                   return launch_pdl(prepare_kernel<decltype(r)::value>, grid, block,
-                                                                     stream, q);
-                                               })
-                                    : launch_pdl(prepare_kernel<0>, grid, block, stream, q);
+    q.rows_used = b.rows_used;
+    q.row_at = b.row_at;
+    cudaError_t err;
+    if (L.targets > 0) {
+        const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, kPrepWarps), 4 * sm_count());
+        err = per_lane(L.targets, [&](auto r) {
+            return launch_pdl(prepare_teacher_kernel<decltype(r)::value>, dim3(static_cast<unsigned>(blocks)),
+                              dim3(32 * kPrepWarps), stream, q);
+        });
+    } else {
+        const int64_t per_block = round_up(ceil_div(L.rows, 4 * sm_count()), kPrepWarps);
+        err = launch_pdl(prepare_rows_kernel, dim3(static_cast<unsigned>(ceil_div(L.rows, per_block))),
+                         dim3(32 * kPrepWarps), stream, q, static_cast<int>(per_block));
+    }
     if (err != cudaSuccess)
         return err;
     for (int64_t col0 = 0; col0 < L.vocab; col0 += b.piece) {
@@ -1540,26 +1719,26 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
         if (!map16(&out, kBf16, b.g, L.rows, cols, b.ldg, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B))
             return cudaErrorInvalidValue;
         Params p{};
+        p.rows_used = b.rows_used;
         p.t_index = b.t_index;
         p.t_prob = b.t_prob;
         p.targets = b.targets;
         p.row_lse2 = b.row_lse2;
         p.row_gain = b.row_gain;
-        err = launch_logits<kGrad, kBf16>(L, b.x_masked, col0, cols, b.grad_bn, b.single, out, p, stream);
-        if (err == cudaSuccess && L.dx)
-            err = launch_dx<kBf16>(L, b, col0, cols, col0 == 0, stream);
-        if (err == cudaSuccess && L.dweight)
-            err = launch_dw<kBf16>(L, b, col0, cols, stream);
+        err = launch_logits<kGrad, kBf16>(L, b.x_used, col0, cols, b.grad_bn, b.single, &out, p, stream);
+        if (err == cudaSuccess)
+            err = launch_back<kBf16>(L, b, col0, cols, stream);
         if (err != cudaSuccess)
             return err;
     }
-    if (L.dx && b.planes) {
-        const int64_t elements = L.rows * L.width;
-        const int64_t plane_blocks = std::min<int64_t>(ceil_div(elements / 8, 256), 8 * sm_count());
-        err = launch_pdl(planes_kernel<kBf16>, dim3(static_cast<unsigned>(plane_blocks)), dim3(256), stream,
+    if (L.dx) {
+        const int64_t threads = std::min<int64_t>(round_up(L.width / 8, 32), 256);
+        const int64_t blocks = std::min<int64_t>(L.rows, 8192 / threads * sm_count());
+        err = launch_pdl(planes_kernel<kBf16>, dim3(static_cast<unsigned>(blocks)),
+                         dim3(static_cast<unsigned>(threads)), stream,
                          static_cast<const float *>(b.dx_planes), static_cast<int>(b.splits),
-                         static_cast<size_t>(elements), static_cast<const float *>(b.inv_gain),
-                         static_cast<uint4 *>(L.dx));
+                         static_cast<int>(L.rows), static_cast<int>(L.width), static_cast<const int *>(b.row_at),
+                         static_cast<const float *>(b.inv_gain), static_cast<uint4 *>(L.dx));
     }
     return err;
 }
