@@ -669,10 +669,12 @@ lffw_status lffw_device_error(int32_t *where) noexcept
 {
     int site = 0;
     cudaError_t err = lffw::read_and_clear_device_error(&site);
-    int vocab_site = 0;
-    if (err == cudaSuccess)
-        err = lffw::read_and_clear_vocab_wait_error(&vocab_site);
-    site = site != 0 ? site : vocab_site;
+    for (const auto read : {lffw::read_and_clear_vocab_wait_error, lffw::read_and_clear_norm_wait_error}) {
+        int other = 0;
+        if (err == cudaSuccess)
+            err = read(&other);
+        site = site != 0 ? site : other;
+    }
     if (where)
         *where = site;
     if (err != cudaSuccess)

@@ -202,8 +202,10 @@ cudaError_t launch_vocab_loss(const VocabLossLaunch &p, cudaStream_t stream);
 cudaError_t launch_vocab_loss_grad(const VocabLossLaunch &p, cudaStream_t stream);
 // 1 when a token outside the vocabulary was met, 0 when none, -1 when it cannot be read.
 int read_and_clear_token_error();
-// The vocabulary kernels' bounded-wait word (see read_and_clear_device_error).
+// The bounded-wait words of the vocabulary and the training norm kernels (see
+// read_and_clear_device_error).
 cudaError_t read_and_clear_vocab_wait_error(int *site);
+cudaError_t read_and_clear_norm_wait_error(int *site);
 
 cudaError_t read_and_clear_device_error(int *site);
 uint64_t launch_count();

@@ -917,11 +917,13 @@ constexpr int kHeadVectors = 5; // 1280 elements of a row per lane group, reques
 // their states, labels, lse and gain g T s.  The others (padding, in a batch of transcripts)
 // take no part in the products, so whatever they hold, NaN included, reaches nothing and costs
 // nothing.  Up to 255 zero rows follow, to the end of a tile, so that what a tile reads there
-// adds nothing.  Each block counts the valid labels before its rows itself (a few KB of reads).
-__global__ void __launch_bounds__(32 * kPrepWarps) prepare_rows_kernel(const Prepare p, int rows_per_block)
+// adds nothing.  Each block counts the valid labels before its rows itself (a few KB of reads),
+// which is why there is one large block per SM.
+constexpr int kRowWarps = 32;
+__global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prepare p, int rows_per_block)
 {
-    __shared__ float warp_max[kPrepWarps];
-    __shared__ int warp_before[kPrepWarps], warp_total[kPrepWarps];
+    __shared__ float warp_max[kRowWarps];
+    __shared__ int warp_before[kRowWarps], warp_total[kRowWarps];
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -931,7 +933,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_rows_kernel(const Pre
     float top = 0.0f;
     int before = 0, total = 0;
 #pragma unroll 8
-    for (int i = threadIdx.x; i < p.t.rows; i += 32 * kPrepWarps) {
+    for (int i = threadIdx.x; i < p.t.rows; i += 32 * kRowWarps) {
         const float g = fabsf(__ldg(p.grad + i));
         const bool used = valid(load_label(p.labels, p.label_bytes, i));
         top = fmaxf(top, used && g < INFINITY ? g : 0.0f);
@@ -953,7 +955,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_rows_kernel(const Pre
     top = 0.0f;
     before = total = 0;
 #pragma unroll
-    for (int i = 0; i < kPrepWarps; ++i) {
+    for (int i = 0; i < kRowWarps; ++i) {
         top = fmaxf(top, warp_max[i]);
         before += warp_before[i];
         total += warp_total[i];
@@ -973,7 +975,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_rows_kernel(const Pre
                 g_token_error = 1;
             p.row_at[first + lane] = valid(mine) ? before + __popc(mask & ((1u << lane) - 1u)) : -1;
         }
-        for (int j = warp; j < 32; j += kPrepWarps) {
+        for (int j = warp; j < 32; j += kRowWarps) {
             if (!(mask >> j & 1u))
                 continue;
             const int row = first + j, to = before + __popc(mask & ((1u << j) - 1u));
@@ -1001,7 +1003,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_rows_kernel(const Pre
         before += __popc(mask);
     }
     const int tail = min(max((total + 255) / 256, 1) * 256, p.t.rows);
-    for (int row = total + blockIdx.x * kPrepWarps + warp; row < tail; row += gridDim.x * kPrepWarps) {
+    for (int row = total + blockIdx.x * kRowWarps + warp; row < tail; row += gridDim.x * kRowWarps) {
         for (int i = lane; i < vectors; i += 32)
             x_used[static_cast<size_t>(row) * vectors + i] = make_uint4(0u, 0u, 0u, 0u);
         if (lane == 0) {
@@ -1204,7 +1206,7 @@ __device__ __forceinline__ void merge_pair(float &mx, float &sum, double &target
 
 // Forward's last step, in a fixed order.  Many rows: 32 rows per block, lane = row (coalesced),
 // warps over the column tiles.
-constexpr int kCombineGroups = 32;
+constexpr int kCombineGroups = 16;
 template <bool kBf16>
 __global__ void __launch_bounds__(32 * kCombineGroups) combine_kernel(const Combine p)
 {
@@ -1222,11 +1224,10 @@ __global__ void __launch_bounds__(32 * kCombineGroups) combine_kernel(const Comb
     s_max[group][lane] = mx;
     s_sum[group][lane] = sum;
     s_t[group][lane] = target;
-    const int mine = blockIdx.x * 32 + group; // this warp's row of the label products
-    if (p.labels && mine < p.rows) {
-        const float z = label_product<kBf16>(p, mine, lane);
+    for (int i = group; p.labels && i < 32 && blockIdx.x * 32 + i < p.rows; i += kCombineGroups) {
+        const float z = label_product<kBf16>(p, blockIdx.x * 32 + i, lane);
         if (lane == 0)
-            s_label[group] = z;
+            s_label[i] = z;
     }
     __syncthreads();
     if (group != 0 || row >= p.rows)
@@ -1259,9 +1260,9 @@ __global__ void __launch_bounds__(32 * kCombineRowWarps) combine_rows_kernel(con
 }
 
 // dx = sum of the fp32 planes (one per K split), in order, times 1 / s; rows that moved come
-// from where they went, rows without a target are zero.  Eight elements per thread, the loads
-// of eight planes in flight; blocks own rows (blockIdx.x, then a grid's stride on).
-template <bool kBf16>
+// from where they went, rows without a target are zero.  Eight elements per thread; blocks own
+// runs of kRows rows, and kRows rows of kPlanes planes are in flight together.
+template <bool kBf16, int kRows, int kPlanes>
 __global__ void __launch_bounds__(256) planes_kernel(const float *planes, int count, int rows, int width,
                                                      const int *row_at, const float *inv_gain, uint4 *dx)
 {
@@ -1270,32 +1271,43 @@ __global__ void __launch_bounds__(256) planes_kernel(const float *planes, int co
     const float inv = *inv_gain;
     const int vectors = width / 8;
     const size_t plane = static_cast<size_t>(rows) * vectors; // in pairs of float4
-    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-        const int from = row_at ? __ldg(row_at + row) : row;
+    const float4 *all = reinterpret_cast<const float4 *>(planes);
+    for (int row0 = blockIdx.x * kRows; row0 < rows; row0 += gridDim.x * kRows) {
+        int from[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+            from[r] = row0 + r >= rows ? -1 : row_at ? __ldg(row_at + row0 + r) : row0 + r;
         for (int i = threadIdx.x; i < vectors; i += blockDim.x) {
-            float f[8] = {};
-            if (from >= 0) {
-                const float4 *src =
-                    reinterpret_cast<const float4 *>(planes) + 2 * (static_cast<size_t>(from) * vectors + i);
-                for (int s = 0; s < count; s += 8) {
-                    float4 lo[8], hi[8];
+            float f[kRows][8] = {};
+            for (int s = 0; s < count; s += kPlanes) {
+                float4 v[kRows][kPlanes][2];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (s + j < count) {
-                            lo[j] = __ldg(src + 2 * plane * (s + j));
-                            hi[j] = __ldg(src + 2 * plane * (s + j) + 1);
+                for (int r = 0; r < kRows; ++r)
+#pragma unroll
+                    for (int j = 0; j < kPlanes; ++j)
+                        if (from[r] >= 0 && s + j < count) {
+                            const float4 *src =
+                                all + 2 * (plane * (s + j) + static_cast<size_t>(from[r]) * vectors + i);
+                            v[r][j][0] = __ldg(src);
+                            v[r][j][1] = __ldg(src + 1);
+                        } else {
+                            v[r][j][0] = v[r][j][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (s + j < count) {
-                            f[0] += lo[j].x, f[1] += lo[j].y, f[2] += lo[j].z, f[3] += lo[j].w;
-                            f[4] += hi[j].x, f[5] += hi[j].y, f[6] += hi[j].z, f[7] += hi[j].w;
-                        }
-                }
+                for (int r = 0; r < kRows; ++r)
+#pragma unroll
+                    for (int j = 0; j < kPlanes; ++j) {
+                        const float4 lo = v[r][j][0], hi = v[r][j][1];
+                        f[r][0] += lo.x, f[r][1] += lo.y, f[r][2] += lo.z, f[r][3] += lo.w;
+                        f[r][4] += hi.x, f[r][5] += hi.y, f[r][6] += hi.z, f[r][7] += hi.w;
+                    }
             }
-            dx[static_cast<size_t>(row) * vectors + i] =
-                make_uint4(pack16(f[0] * inv, f[1] * inv, kBf16), pack16(f[2] * inv, f[3] * inv, kBf16),
-                           pack16(f[4] * inv, f[5] * inv, kBf16), pack16(f[6] * inv, f[7] * inv, kBf16));
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+                if (row0 + r < rows)
+                    dx[static_cast<size_t>(row0 + r) * vectors + i] =
+                        make_uint4(pack16(f[r][0] * inv, f[r][1] * inv, kBf16), pack16(f[r][2] * inv, f[r][3] * inv, kBf16),
+                                   pack16(f[r][4] * inv, f[r][5] * inv, kBf16), pack16(f[r][6] * inv, f[r][7] * inv, kBf16));
         }
     }
 }
@@ -1707,9 +1719,9 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
                               dim3(32 * kPrepWarps), stream, q);
         });
     } else {
-        const int64_t per_block = round_up(ceil_div(L.rows, 4 * sm_count()), kPrepWarps);
+        const int64_t per_block = round_up(ceil_div(L.rows, sm_count()), kRowWarps);
         err = launch_pdl(prepare_rows_kernel, dim3(static_cast<unsigned>(ceil_div(L.rows, per_block))),
-                         dim3(32 * kPrepWarps), stream, q, static_cast<int>(per_block));
+                         dim3(32 * kRowWarps), stream, q, static_cast<int>(per_block));
     }
     if (err != cudaSuccess)
         return err;
@@ -1732,10 +1744,12 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
             return err;
     }
     if (L.dx) {
+        // Few planes: four rows at a time; many (few rows): eight planes of one.
+        const bool few = b.splits <= 2;
         const int64_t threads = std::min<int64_t>(round_up(L.width / 8, 32), 256);
-        const int64_t blocks = std::min<int64_t>(L.rows, 8192 / threads * sm_count());
-        err = launch_pdl(planes_kernel<kBf16>, dim3(static_cast<unsigned>(blocks)),
-                         dim3(static_cast<unsigned>(threads)), stream,
+        const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, few ? 4 : 1), 4096 / threads * sm_count());
+        const auto kernel = few ? planes_kernel<kBf16, 4, 1> : planes_kernel<kBf16, 1, 8>;
+        err = launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(static_cast<unsigned>(threads)), stream,
                          static_cast<const float *>(b.dx_planes), static_cast<int>(b.splits),
                          static_cast<int>(L.rows), static_cast<int>(L.width), static_cast<const int *>(b.row_at),
                          static_cast<const float *>(b.inv_gain), static_cast<uint4 *>(L.dx));
