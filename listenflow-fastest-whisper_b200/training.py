@@ -18,7 +18,6 @@ allocated on it.  Every byte of arithmetic runs in liblffw_b200.so.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
@@ -30,13 +29,23 @@ IGNORE_INDEX = -100
 
 _DTYPES = {torch.float16: native.DT_HALF, torch.bfloat16: native.DT_BF16}
 _TEACHER_DTYPES = {**_DTYPES, torch.float32: native.DT_FLOAT}
-_HERE = contextlib.nullcontext()
+
+
+# The current device's index and its current stream's handle, without the objects that
+# torch.cuda wraps them in (a tenth of a small call's host time).
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _elsewhere(device: torch.device, stream) -> bool:
+    """Whether a call has to make another device or stream current first (see _scope)."""
+    return stream is not None or device.index != _current_device()
 
 
 def _scope(device: torch.device, stream):
-    """Makes `device` and `stream` current (allocations follow the current stream)."""
+    """Makes `device` and `stream` current: allocations follow the current stream."""
     if stream is None:
-        return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        return torch.cuda.device(device)
     if not isinstance(stream, torch.cuda.Stream):
         handle = int(stream)
         stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
@@ -64,11 +73,6 @@ def _vector(t: torch.Tensor, dtypes, count: int, device: torch.device, name: str
         raise ValueError(f"{name} must be a contiguous {kinds} tensor [{count}] on {device}")
 
 
-# The current stream's handle by device index, without a Stream object around it (a tenth of
-# a small call's host time).
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
 def _run(call, args, name: str, device: torch.device) -> None:
     status = call(ctypes.byref(args), _raw_stream(device.index))
     if status:
@@ -93,16 +97,18 @@ def layer_norm_forward(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor,
     _vector(beta, _FLOAT, cols, device, "beta")
     if residual is not None:
         _like(residual, x, "residual", "x")
-    with _scope(device, stream):
-        total = x if residual is None else torch.empty_like(x)
-        y = torch.empty_like(x)
-        stats = gamma.new_empty((2, rows))
-        if rows:
-            a = native.LayerNormTrainArgs(
-                ctypes.sizeof(native.LayerNormTrainArgs), rows, cols, dtype, x.data_ptr(),
-                None if residual is None else residual.data_ptr(), None if residual is None else total.data_ptr(),
-                gamma.data_ptr(), beta.data_ptr(), eps, y.data_ptr(), stats.data_ptr())
-            _run(native.library().lffw_layer_norm_train, a, "lffw_layer_norm_train", device)
+    if _elsewhere(device, stream):
+        with _scope(device, stream):
+            return layer_norm_forward(x, gamma, beta, eps, residual=residual)
+    total = x if residual is None else torch.empty_like(x)
+    y = torch.empty_like(x)
+    stats = gamma.new_empty((2, rows))
+    if rows:
+        a = native.LayerNormTrainArgs(
+            ctypes.sizeof(native.LayerNormTrainArgs), rows, cols, dtype, x.data_ptr(),
+            None if residual is None else residual.data_ptr(), None if residual is None else total.data_ptr(),
+            gamma.data_ptr(), beta.data_ptr(), eps, y.data_ptr(), stats.data_ptr())
+        _run(native.library().lffw_layer_norm_train, a, "lffw_layer_norm_train", device)
     return total, y, stats
 
 
@@ -124,24 +130,26 @@ def layer_norm_backward(dy: torch.Tensor, total: torch.Tensor, gamma: torch.Tens
         raise ValueError("stats must be layer_norm_forward's float32 [2, rows]")
     if not want_dx and not want_params:
         raise ValueError("nothing to compute: want_dx and want_params are both false")
-    with _scope(device, stream):
-        dx = torch.empty_like(total) if want_dx else None
-        dgamma = dbeta = workspace = None
-        size = 0
-        if not rows:
-            return (dx, torch.zeros_like(gamma), torch.zeros_like(gamma)) if want_params else (dx, None, None)
-        lib = native.library()
-        if want_params:
-            dgamma, dbeta = gamma.new_empty(cols), gamma.new_empty(cols)
-            size = lib.lffw_layer_norm_grad_workspace(rows, cols)
-            if size > 0:
-                workspace = gamma.new_empty(size // 4)
-        a = native.LayerNormGradArgs(
-            ctypes.sizeof(native.LayerNormGradArgs), rows, cols, dtype, dy.data_ptr(), total.data_ptr(),
-            gamma.data_ptr(), stats.data_ptr(), None if dsum is None else dsum.data_ptr(),
-            dx.data_ptr() if want_dx else None, dgamma.data_ptr() if want_params else None,
-            dbeta.data_ptr() if want_params else None, None if workspace is None else workspace.data_ptr(), size)
-        _run(lib.lffw_layer_norm_grad, a, "lffw_layer_norm_grad", device)
+    if _elsewhere(device, stream):
+        with _scope(device, stream):
+            return layer_norm_backward(dy, total, gamma, stats, dsum=dsum, want_dx=want_dx, want_params=want_params)
+    dx = torch.empty_like(total) if want_dx else None
+    dgamma = dbeta = workspace = None
+    size = 0
+    if not rows:
+        return (dx, torch.zeros_like(gamma), torch.zeros_like(gamma)) if want_params else (dx, None, None)
+    lib = native.library()
+    if want_params:
+        dgamma, dbeta = gamma.new_empty(cols), gamma.new_empty(cols)
+        size = lib.lffw_layer_norm_grad_workspace(rows, cols)
+        if size > 0:
+            workspace = gamma.new_empty(size // 4)
+    a = native.LayerNormGradArgs(
+        ctypes.sizeof(native.LayerNormGradArgs), rows, cols, dtype, dy.data_ptr(), total.data_ptr(),
+        gamma.data_ptr(), stats.data_ptr(), None if dsum is None else dsum.data_ptr(),
+        dx.data_ptr() if want_dx else None, dgamma.data_ptr() if want_params else None,
+        dbeta.data_ptr() if want_params else None, None if workspace is None else workspace.data_ptr(), size)
+    _run(lib.lffw_layer_norm_grad, a, "lffw_layer_norm_grad", device)
     return dx, dgamma, dbeta
 
 
@@ -191,13 +199,15 @@ def _workspace(a: native.VocabLossArgs, x: torch.Tensor, grad: int) -> torch.Ten
 
 def _loss_forward(a: native.VocabLossArgs, x: torch.Tensor, stream):
     device, rows = x.device, a.rows
-    with _scope(device, stream):
-        losses = torch.empty(rows, dtype=torch.float32, device=device)
-        lse = torch.empty_like(losses)
-        if rows:
-            a.losses, a.lse = losses.data_ptr(), lse.data_ptr()
-            workspace = _workspace(a, x, 0)  # noqa: F841 (freed after the call is queued)
-            _run(native.library().lffw_vocab_loss, a, "lffw_vocab_loss", device)
+    if _elsewhere(device, stream):
+        with _scope(device, stream):
+            return _loss_forward(a, x, None)
+    losses = torch.empty(rows, dtype=torch.float32, device=device)
+    lse = torch.empty_like(losses)
+    if rows:
+        a.losses, a.lse = losses.data_ptr(), lse.data_ptr()
+        workspace = _workspace(a, x, 0)  # noqa: F841 (freed after the call is queued)
+        _run(native.library().lffw_vocab_loss, a, "lffw_vocab_loss", device)
     return losses, lse
 
 
@@ -208,16 +218,18 @@ def _loss_backward(a: native.VocabLossArgs, x: torch.Tensor, weight: torch.Tenso
     _vector(dloss, _FLOAT, rows, device, "dloss")
     if not want_dx and not want_dweight:
         raise ValueError("nothing to compute: want_dx and want_dweight are both false")
-    with _scope(device, stream):
-        dx = torch.empty_like(x) if want_dx else None
-        if not rows:
-            return dx, torch.zeros_like(weight) if want_dweight else None
-        dweight = torch.empty_like(weight) if want_dweight else None
-        a.lse, a.dloss = lse.data_ptr(), dloss.data_ptr()
-        a.dx = dx.data_ptr() if want_dx else None
-        a.dweight = dweight.data_ptr() if want_dweight else None
-        workspace = _workspace(a, x, 1)  # noqa: F841 (freed after the call is queued)
-        _run(native.library().lffw_vocab_loss_grad, a, "lffw_vocab_loss_grad", device)
+    if _elsewhere(device, stream):
+        with _scope(device, stream):
+            return _loss_backward(a, x, weight, lse, dloss, want_dx, want_dweight, None)
+    dx = torch.empty_like(x) if want_dx else None
+    if not rows:
+        return dx, torch.zeros_like(weight) if want_dweight else None
+    dweight = torch.empty_like(weight) if want_dweight else None
+    a.lse, a.dloss = lse.data_ptr(), dloss.data_ptr()
+    a.dx = dx.data_ptr() if want_dx else None
+    a.dweight = dweight.data_ptr() if want_dweight else None
+    workspace = _workspace(a, x, 1)  # noqa: F841 (freed after the call is queued)
+    _run(native.library().lffw_vocab_loss_grad, a, "lffw_vocab_loss_grad", device)
     return dx, dweight
 
 
