@@ -19,6 +19,9 @@ end-of-text are ignored by the caller).  The cache is a fixed-capacity fp16 buff
 stream, also each new token's position) stay on the device, so one CUDA graph of
 a step replays for every step.  A plan serves at most 32 streams (the small-M
 tensor-core linears); more streams use several plans.
+
+score and divergence judge given transcripts by the same plan, teacher-forced: the
+token losses of training.py over all positions' final states at once.
 """
 
 from __future__ import annotations
@@ -32,6 +35,7 @@ import torch
 
 from . import _native as native
 from . import fp8
+from . import training
 from .encoder import NEG_ZERO_HALF
 
 MAX_STREAMS = 32
@@ -339,6 +343,65 @@ class Decoder:
         st = fp8._stream(stream)
         for name, call in self._calls:
             native.check(call(st), name)
+
+
+    def final_states(self, transcripts: torch.Tensor, start_token: int = SOT,
+                     ignore_index: int = training.IGNORE_INDEX) -> torch.Tensor:
+        """Teacher-forced decoding on the current stream: transcripts int32 [streams, length]
+        (length up to the cache's capacity and the position table) on the plan's device, padded with `ignore_index`.  Returns the
+        final states fp16 [length, streams, d] that predict each of their tokens: the state at
+        position t has read start_token and tokens 0 .. t - 1.  Leaves the caches holding the
+        transcripts' tokens but the last."""
+        c, s = self.config, self.streams
+        if (transcripts.dtype != torch.int32 or transcripts.dim() != 2 or transcripts.shape[0] != s
+                or transcripts.device != self.tokens.device
+                or not 1 <= transcripts.shape[1] <= min(self.capacity, c.positions)):
+            raise ValueError(f"transcripts must be int32 [{s}, 1 to {min(self.capacity, c.positions)}] on "
+                             f"{self.tokens.device}")
+        length = transcripts.shape[1]
+        # Padding is read as end of text; what it leads to is ignored by the losses.
+        pad = min(EOT, c.vocab - 1)
+        read = torch.where(transcripts == ignore_index, pad, transcripts).to(torch.int32).t().contiguous()
+        out = torch.empty((length, s, c.d_model), dtype=torch.float16, device=transcripts.device)
+        st = fp8._stream(None)
+        self.reset(start_token)
+        for t in range(length):
+            if t:
+                self.tokens.copy_(read[t - 1])
+            for name, call in self._calls[:-2]:  # neither the logits nor the choice
+                native.check(call(st), name)
+            out[t].copy_(self.states)
+            self.lengths += 1
+        return out
+
+    def score(self, transcripts: torch.Tensor, start_token: int = SOT,
+              ignore_index: int = training.IGNORE_INDEX) -> torch.Tensor:
+        """-log p(token | the tokens before it) of given transcripts [streams, length] (see
+        final_states), fp32, 0 for padding: with its sum a transcript's log-likelihood, with
+        its mean what the avg_logprob threshold of a decode is held against."""
+        states = self.final_states(transcripts, start_token, ignore_index)
+        labels = transcripts.t().contiguous().view(-1)
+        losses, _ = training.cross_entropy_forward(states.view(-1, self.config.d_model), self.weights.token_table,
+                                                   labels, ignore_index=ignore_index)
+        return losses.view(transcripts.shape[1], self.streams).t()
+
+    def divergence(self, transcripts: torch.Tensor, teacher_tokens: torch.Tensor, teacher_logits: torch.Tensor, *,
+                   temperature: float = 1.0, start_token: int = SOT,
+                   ignore_index: int = training.IGNORE_INDEX) -> torch.Tensor:
+        """T^2 KL(teacher || this decoder) per token of given transcripts, fp32 [streams,
+        length], 0 for padding, from a teacher's best logits [streams, length, k] (int32 tokens,
+        fp16/bf16/fp32 logits): how far quantisation has moved a decoder from the one it was
+        made of, token by token."""
+        if teacher_tokens.shape[:2] != transcripts.shape or teacher_logits.shape != teacher_tokens.shape:
+            raise ValueError("teacher_tokens and teacher_logits must be [streams, length, k] like transcripts")
+        states = self.final_states(transcripts, start_token, ignore_index)
+        k = teacher_tokens.shape[2]
+        tokens = torch.where((transcripts == ignore_index).unsqueeze(2), -1, teacher_tokens).to(torch.int32)
+        losses, _ = training.distillation_forward(
+            states.view(-1, self.config.d_model), self.weights.token_table,
+            tokens.transpose(0, 1).reshape(-1, k).contiguous(),
+            teacher_logits.transpose(0, 1).reshape(-1, k).contiguous(), temperature=temperature)
+        return losses.view(transcripts.shape[1], self.streams).t()
 
 
 def calibrate(weights: DecoderWeights, cross_kv: torch.Tensor, streams: int, steps: int,

@@ -297,12 +297,11 @@ def _guard_capture(*inputs: torch.Tensor | None) -> list:
     lives as long as a graph holds it, and so does the mark left on it here.  Returns the
     accumulators, for the caller to hold until the new graph does."""
     accumulators = []
-    if not torch.is_grad_enabled():
+    leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf and t.is_cuda]
+    if not leaves or not torch.is_grad_enabled():
         return accumulators
     capturing = torch.cuda.is_current_stream_capturing()
-    for leaf in inputs:
-        if leaf is None or not leaf.requires_grad or not leaf.is_leaf:
-            continue
+    for leaf in leaves:
         accumulators.append(torch.autograd.graph.get_gradient_edge(leaf).node)
         mark = accumulators[-1].metadata
         stream = torch.cuda.current_stream(leaf.device).cuda_stream
