@@ -487,8 +487,8 @@ LFFW_FP8_API lffw_status lffw_layer_norm_grad(const lffw_layer_norm_grad_args *a
  * G is formed piece by piece over the vocabulary and held in 16 bits (scaled by a power of
  * two so that fp16 neither overflows nor loses small probabilities); sums are fp32.
  * workspace holds lffw_vocab_loss_workspace(args, 0 for the loss, 1 for the gradients)
- * bytes (-1 for invalid arguments; it depends on the shape, the targets and, for the
- * gradients, on whether dx is set, not on the contents).
+ * bytes (-1 for invalid arguments; it depends on the current device, the shape, the number
+ * of targets and, for the gradients, on which of dx and dweight are set, never on contents).
  * Requirements: 1 <= rows <= 2^22; 1 <= vocab <= 2^22; 8 <= width <= 2^16, width % 8 == 0;
  * 16-byte aligned x, weight, dx, dweight; a workspace on a 256-byte boundary;
  * temperature in [2^-10, 2^10], exactly 1 with labels. */

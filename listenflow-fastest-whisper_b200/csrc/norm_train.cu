@@ -409,8 +409,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Params p
     auto load_stats = [&](int64_t row0) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            next_mean[i] = row0 + i < p.rows ? __ldg(p.stats + row0 + i) : 0.0f;
-            next_rstd[i] = row0 + i < p.rows ? __ldg(p.stats + p.rows + row0 + i) : 0.0f;
+            next_mean[i] = row0 + i < p.rows ? p.stats[row0 + i] : 0.0f;
+            next_rstd[i] = row0 + i < p.rows ? p.stats[p.rows + row0 + i] : 0.0f;
         }
     };
     load_stats(first);

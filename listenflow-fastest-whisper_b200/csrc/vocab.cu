@@ -271,11 +271,13 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
         }
         mbar_init(bar_drain, 1);
         fence_barrier_init();
-        prefetch_tensor_map(&tm_a);
-        prefetch_tensor_map(&tm_b);
-        if (MODE != kStats)
-            prefetch_tensor_map(&tm_out);
-        if (MODE == kBack) {
+        if (MODE != kBack || p.dx_splits > 0) {
+            prefetch_tensor_map(&tm_a);
+            prefetch_tensor_map(&tm_b);
+            if (MODE != kStats)
+                prefetch_tensor_map(&tm_out);
+        }
+        if (MODE == kBack && p.dw_tiles > 0) {
             prefetch_tensor_map(&tm_a2);
             prefetch_tensor_map(&tm_b2);
             prefetch_tensor_map(&tm_out2);
@@ -934,7 +936,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
     int before = 0, total = 0;
 #pragma unroll 8
     for (int i = threadIdx.x; i < p.t.rows; i += 32 * kRowWarps) {
-        const float g = fabsf(__ldg(p.grad + i));
+        const float g = fabsf(p.grad[i]);
         const bool used = valid(load_label(p.labels, p.label_bytes, i));
         top = fmaxf(top, used && g < INFINITY ? g : 0.0f);
         before += used && i < begin;
@@ -985,13 +987,13 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
 #pragma unroll
             for (int i = 0; i < kHeadVectors; ++i)
                 if (lane + 32 * i < vectors)
-                    head[i] = __ldg(src + lane + 32 * i);
+                    head[i] = src[lane + 32 * i];
 #pragma unroll
             for (int i = 0; i < kHeadVectors; ++i)
                 if (lane + 32 * i < vectors)
                     dst[lane + 32 * i] = head[i];
             for (int i = lane + 32 * kHeadVectors; i < vectors; i += 32)
-                dst[i] = __ldg(src + i);
+                dst[i] = src[i];
             const int64_t label = __shfl_sync(0xffffffffu, mine, j);
             if (lane == 0) {
                 p.t.index[to] = static_cast<int32_t>(label);
@@ -1030,7 +1032,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
     float top = 0.0f;
 #pragma unroll 8
     for (int i = threadIdx.x; i < p.t.rows; i += 32 * kPrepWarps) {
-        const float g = fabsf(__ldg(p.grad + i));
+        const float g = fabsf(p.grad[i]);
         top = fmaxf(top, g < INFINITY ? g : 0.0f);
     }
 #pragma unroll
@@ -1055,7 +1057,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
 #pragma unroll
         for (int i = 0; i < kHeadVectors; ++i)
             if (lane + 32 * i < vectors)
-                head[i] = __ldg(src + lane + 32 * i);
+                head[i] = src[lane + 32 * i];
         double entropy, total;
         const bool any = sort_targets<R>(p.t, row, lane, probs[warp], entropy, total);
         if (lane == 0) {
@@ -1067,7 +1069,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
             if (lane + 32 * i < vectors)
                 dst[lane + 32 * i] = any ? head[i] : make_uint4(0u, 0u, 0u, 0u);
         for (int i = lane + 32 * kHeadVectors; i < vectors; i += 32)
-            dst[i] = any ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+            dst[i] = any ? src[i] : make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
@@ -1123,7 +1125,7 @@ __device__ __forceinline__ float label_product(const Combine &p, int row, int la
         const uint4 *b = static_cast<const uint4 *>(p.weight) + static_cast<size_t>(label) * (p.width / 8);
 #pragma unroll 5
         for (int i = lane; i < p.width / 8; i += 32)
-            z = dot16<kBf16>(__ldg(a + i), __ldg(b + i), z);
+            z = dot16<kBf16>(a[i], b[i], z);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1)
@@ -1173,10 +1175,10 @@ __device__ __forceinline__ void merge_tiles(const Combine &p, int row, int first
             v[j] = t[j] = 0.0f;
             if (i < p.slices) {
                 const size_t at = static_cast<size_t>(i) * p.rows + row;
-                m[j] = __ldg(p.part_max + at);
-                v[j] = __ldg(p.part_sum + at);
+                m[j] = p.part_max[at];
+                v[j] = p.part_sum[at];
                 if (p.part_t)
-                    t[j] = __ldg(p.part_t + at);
+                    t[j] = p.part_t[at];
             }
         }
         float next = mx;
@@ -1276,7 +1278,7 @@ __global__ void __launch_bounds__(256) planes_kernel(const float *planes, int co
         int from[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r)
-            from[r] = row0 + r >= rows ? -1 : row_at ? __ldg(row_at + row0 + r) : row0 + r;
+            from[r] = row0 + r >= rows ? -1 : row_at ? row_at[row0 + r] : row0 + r;
         for (int i = threadIdx.x; i < vectors; i += blockDim.x) {
             float f[kRows][8] = {};
             for (int s = 0; s < count; s += kPlanes) {
@@ -1288,8 +1290,8 @@ __global__ void __launch_bounds__(256) planes_kernel(const float *planes, int co
                         if (from[r] >= 0 && s + j < count) {
                             const float4 *src =
                                 all + 2 * (plane * (s + j) + static_cast<size_t>(from[r]) * vectors + i);
-                            v[r][j][0] = __ldg(src);
-                            v[r][j][1] = __ldg(src + 1);
+                            v[r][j][0] = src[0];
+                            v[r][j][1] = src[1];
                         } else {
                             v[r][j][0] = v[r][j][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         }
@@ -1328,7 +1330,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int64_t kSingleRows = 128;
 
 // Up to this many rows the forward's last step takes a warp per row (20 rows: 10 us with 32
-// rows per block, TODO us with a warp each); above, its strided reads cost more than they save.
+// rows per block, 4.9 us with a warp each); above, its strided reads cost more than they save.
 constexpr int64_t kCombineRows = 1024;
 
 // Bytes of one piece of G.
