@@ -491,7 +491,7 @@ LFFW_FP8_API lffw_status lffw_layer_norm_grad(const lffw_layer_norm_grad_args *a
  * of targets and, for the gradients, on which of dx and dweight are set, never on contents).
  * Requirements: 1 <= rows <= 2^22; 1 <= vocab <= 2^22; 8 <= width <= 2^16, width % 8 == 0;
  * 16-byte aligned x, weight, dx, dweight; a workspace on a 256-byte boundary;
- * temperature in [2^-10, 2^10], exactly 1 with labels. */
+ * temperature in [2^-6, 2^6], exactly 1 with labels. */
 typedef struct lffw_vocab_loss_args {
     size_t struct_size; /* sizeof(lffw_vocab_loss_args) */
     int64_t rows, width, vocab;

@@ -63,7 +63,7 @@ lffw_status validate_vocab(const lffw_vocab_loss_args *a)
         return LFFW_INVALID_ARGUMENT;
     if (!aligned(a->teacher_logits, a->teacher_dtype == LFFW_DT_FLOAT ? 4 : 2))
         return LFFW_INVALID_ARGUMENT;
-    return std::isfinite(a->temperature) && a->temperature >= 0x1p-10f && a->temperature <= 0x1p10f
+    return std::isfinite(a->temperature) && a->temperature >= 0x1p-6f && a->temperature <= 0x1p6f
                ? LFFW_SUCCESS
                : LFFW_INVALID_ARGUMENT;
 }

@@ -27,6 +27,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -813,7 +814,7 @@ __device__ __forceinline__ bool sort_targets(const Targets &t, int row, int lane
     for (int i = 0; i < R; ++i) {
         const int j = lane + 32 * i;
         token[i] = j < t.count ? t.tokens[base + j] : -1;
-        z[i] = j < t.count ? load_float(t.logits, t.logit_type, base + j) * t.inv_temperature : 0.0f;
+        z[i] = j < t.count ? load_float(t.logits, t.logit_type, base + j) : 0.0f;
     }
     uint32_t key[R];
     float top = -INFINITY;
@@ -823,6 +824,9 @@ __device__ __forceinline__ bool sort_targets(const Targets &t, int row, int lane
         if (token[i] >= t.vocab)
             g_token_error = 1;
         const bool valid = token[i] >= 0 && token[i] < t.vocab && z[i] != -INFINITY;
+        // A finite logit stays finite: the lowest value of a type masks nothing.
+        const float scaled = z[i] * t.inv_temperature;
+        z[i] = isinf(scaled) && !isinf(z[i]) ? copysignf(FLT_MAX, z[i]) : scaled;
         key[i] = valid ? (static_cast<uint32_t>(token[i]) << 8) | static_cast<uint32_t>(lane + 32 * i) : kNone;
         z[i] = valid ? z[i] : -INFINITY;
         has |= valid;

@@ -182,8 +182,8 @@ def _with_teacher(a: native.VocabLossArgs, x: torch.Tensor, tokens: torch.Tensor
     if (logits.dtype not in _TEACHER_DTYPES or logits.shape != tokens.shape or logits.device != x.device
             or not logits.is_contiguous()):
         raise ValueError("teacher_logits must be a contiguous float16, bfloat16 or float32 tensor like teacher_tokens")
-    if not 2.0 ** -10 <= temperature <= 2.0 ** 10:
-        raise ValueError("temperature must lie in [2^-10, 2^10]")
+    if not 2.0 ** -6 <= temperature <= 2.0 ** 6:
+        raise ValueError("temperature must lie in [2^-6, 2^6]")
     a.teacher_entries, a.teacher_dtype = tokens.shape[1], _TEACHER_DTYPES[logits.dtype]
     a.teacher_tokens, a.teacher_logits, a.temperature = tokens.data_ptr(), logits.data_ptr(), temperature
 

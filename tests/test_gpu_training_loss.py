@@ -191,6 +191,61 @@ def test_rows_without_teacher_entries(training):
     assert ref.worst(dx, e_dx, b_dx) <= 1 and ref.worst(dw, e_dw, b_dw) <= 1
 
 
+@pytest.mark.parametrize("n", [50, 400])
+def test_ignored_token_of_the_vocabulary(training, n):
+    """ignore_index may be a token: its rows are ignored, its column of the softmax stays."""
+    g, x, w, dloss = operands(n, 64, 300, torch.float16)
+    labels = torch.randint(8, (n,), generator=g, device="cuda")
+    compare(lambda: training.cross_entropy_forward(x, w, labels, ignore_index=5),
+            lambda lse: training.cross_entropy_backward(x, w, labels, lse, dloss, ignore_index=5),
+            x, w, dloss, ref.label_targets(labels, 300, 5))
+
+
+@pytest.mark.parametrize("temperature", [2.0 ** -6, 2.0 ** 6])
+def test_extreme_temperatures(training, temperature):
+    """Both ends of the range, with logits that leave fp32's range when divided by it."""
+    n, d, vocab, k = 70, 64, 500, 6
+    g, x, w, dloss = operands(n, d, vocab, torch.bfloat16, scale=0.02)
+    tokens = torch.randint(vocab, (n, k), generator=g, device="cuda", dtype=torch.int32)
+    logits = torch.randn((n, k), generator=g, device="cuda")
+    logits[:10] = torch.finfo(torch.float32).min
+    logits[20, 2] = torch.finfo(torch.float32).max
+    clipped = torch.where(logits.abs() > 1e30, logits.sign() * 1e30, logits)  # the same softmax in 64 bits
+    compare(lambda: training.distillation_forward(x, w, tokens, logits, temperature=temperature),
+            lambda lse: training.distillation_backward(x, w, tokens, logits, lse, dloss, temperature=temperature),
+            x, w, dloss, ref.teacher_targets(tokens, clipped, vocab, temperature), temperature, k)
+
+
+def test_offsets_past_32_bits(training):
+    """A table of more than 2^31 elements: tokens at both of its ends."""
+    n, d, vocab = 5, 1280, 1_700_000
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.randn((vocab, d), generator=g, device="cuda", dtype=torch.bfloat16)
+    w *= 0.02
+    x = torch.randn((n, d), generator=g, device="cuda").to(torch.bfloat16)
+    labels = torch.tensor([0, vocab - 1, 1_677_721, 1_677_722, 5], device="cuda")
+    dloss = torch.tensor([1.0, 2.0, 0.5, 1.5, -1.0], device="cuda")
+    losses, lse = training.cross_entropy_forward(x, w, labels)
+    dx, dw = training.cross_entropy_backward(x, w, labels, lse, dloss)
+    z = torch.cat([x.double() @ part.double().t() for part in w.split(200_000)], 1)
+    e_lse = torch.logsumexp(z, 1)
+    rows = torch.arange(n, device="cuda")
+    off = ref.logit_bound(x, w[:1000]) * 1.5 + 2.0 ** -16  # rows of the table are alike
+    assert ((lse - e_lse).abs() <= off).all() and ((losses - (e_lse - z[rows, labels])).abs() <= 2 * off).all()
+    p = (z - e_lse.unsqueeze(1)).exp()
+    p[rows, labels] -= 1
+    p *= dloss.double().unsqueeze(1)
+    e_dx = sum(part @ rows_.double() for part, rows_ in zip(p.split(200_000, 1), w.split(200_000)))
+    # G's half step and the logits' error, over the products' magnitudes; one rounding at the end.
+    share = 2.0 ** -9 + torch.expm1(3 * off).max() + vocab * 2 * ref.U32
+    mag = sum(part.abs() @ rows_.double().abs() for part, rows_ in zip(p.split(200_000, 1), w.split(200_000)))
+    assert ((dx.double() - e_dx).abs() <= share * mag + ref.rounding(e_dx.abs(), torch.bfloat16)).all()
+    for part in (slice(0, 1000), slice(1_677_700, 1_678_700), slice(vocab - 1000, vocab)):
+        e_dw = p[:, part].t() @ x.double()
+        mag = p[:, part].abs().t() @ x.double().abs()
+        assert ((dw[part].double() - e_dw).abs() <= share * mag + ref.rounding(e_dw.abs(), torch.bfloat16) + 1e-9).all()
+
+
 def test_all_rows_ignored(training):
     g, x, w, dloss = operands(33, 64, 200, torch.bfloat16)
     labels = torch.full((33,), -100, device="cuda")

@@ -47,7 +47,8 @@ def check(training, s, eps=1e-5):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("rows,cols", [(1, 8), (2, 264), (3, 256), (20, 1280), (447, 384), (1001, 512), (333, 1000),
-                                       (7, 4096), (2500, 768), (6001, 1280), (700, 2560), (149, 4088)])
+                                       (7, 4096), (2500, 768), (6001, 1280), (700, 2560), (149, 4088), (1001, 4096),
+                                       (5003, 8), (9001, 256), (4444, 520)])
 def test_against_64_bits(training, rows, cols, dtype, residual):
     check(training, make(rows, cols, dtype, residual))
 
@@ -56,6 +57,29 @@ def test_against_64_bits(training, rows, cols, dtype, residual):
 def test_row_counts_around_a_full_step(training, rows):
     """Around 148 SMs x 4 groups x 1, 2 and 4 rows, where the rows per step and the tail change."""
     check(training, make(rows, 1280, torch.float16, True, seed=3))
+
+
+def test_offsets_past_32_bits(training):
+    """2^31 elements and more: the last rows against 64 bits, the column sums against the sum of
+    two halves of the rows."""
+    rows, cols = (1 << 31) // 1280 + 1000, 1280
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn((rows, cols), generator=g, device="cuda", dtype=torch.bfloat16)
+    dy = torch.randn((rows, cols), generator=g, device="cuda", dtype=torch.bfloat16)
+    gamma, beta = torch.rand(cols, generator=g, device="cuda") + 0.5, torch.randn(cols, generator=g, device="cuda")
+    total, y, stats = training.layer_norm_forward(x, gamma, beta)
+    dx, dgamma, dbeta = training.layer_norm_backward(dy, total, gamma, stats)
+    last = slice(rows - 700, rows)
+    _, e_y, mean, rstd = ref.layer_norm(x[last], gamma, beta, 1e-5)
+    assert ref.worst(y[last], e_y, ref.layer_norm_bound(x[last], gamma, beta, e_y, mean, rstd)) <= 1
+    e_dx, _, _ = ref.layer_norm_grads(dy[last], x[last], gamma, mean, rstd)
+    b_dx, _, _ = ref.layer_norm_grad_bounds(dy[last], x[last], gamma, mean, rstd, e_dx)
+    assert ref.worst(dx[last], e_dx, b_dx) <= 1
+    halves = [training.layer_norm_backward(dy[part], x[part], gamma, stats[:, part].contiguous(), want_dx=False)
+              for part in (slice(0, rows // 2), slice(rows // 2, rows))]
+    # Sums of up to `rows` terms of size about 1 (each at most 32), in two orders.
+    for whole, first, second in ((dgamma, halves[0][1], halves[1][1]), (dbeta, halves[0][2], halves[1][2])):
+        assert ((whole - first - second).abs() <= 2 * rows * ref.U32 * 3 * rows ** 0.5).all()
 
 
 def test_rows_behind_the_last_are_left(training):

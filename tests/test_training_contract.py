@@ -71,7 +71,7 @@ SHARED = [
     (TEACHER, {"teacher_entries": 257}), (TEACHER, {"teacher_tokens": None}), (TEACHER, {"teacher_tokens": 0x30002}),
     (TEACHER, {"teacher_logits": None}), (TEACHER, {"teacher_logits": 0x38002}), (TEACHER, {"teacher_dtype": 2}),
     (TEACHER, {"temperature": 0.0}), (TEACHER, {"temperature": -1.0}), (TEACHER, {"temperature": float("nan")}),
-    (TEACHER, {"temperature": float("inf")}), (TEACHER, {"temperature": 2.0**11}),
+    (TEACHER, {"temperature": float("inf")}), (TEACHER, {"temperature": 2.0**6.5}), (TEACHER, {"temperature": 2.0**-6.5}),
 ]
 
 
