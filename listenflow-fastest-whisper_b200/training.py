@@ -140,7 +140,7 @@ def layer_norm_backward(dy: torch.Tensor, total: torch.Tensor, gamma: torch.Tens
         return (dx, torch.zeros_like(gamma), torch.zeros_like(gamma)) if want_params else (dx, None, None)
     lib = native.library()
     if want_params:
-        dgamma, dbeta = gamma.new_empty(cols), gamma.new_empty(cols)
+        dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
         size = lib.lffw_layer_norm_grad_workspace(rows, cols)
         if size > 0:
             workspace = gamma.new_empty(size // 4)
