@@ -96,11 +96,78 @@ struct Cfg {
     static_assert((2 * kStages + 5) * 8 + 8 <= kBarBytes, "barrier area");
 };
 
+// The backward's shape, decided on the device once the rows that have a target are counted.
+struct BackShape {
+    int rows;       // of G and x_used
+    int kb_per;     // K blocks of one split of dx
+    int splits;     // planes of dx
+    int plane_rows; // rows from one plane to the next: rows, rounded up to a store's 32
+};
+
+// What the choice of dx's splits depends on.
+struct BackCosts {
+    int kbs, pieces;         // K blocks of dx in a piece, and pieces
+    int n_tiles, dw_m_tiles; // tiles across x's width, and of dW down a piece (0: no dW)
+    int units;               // CTA pairs
+    int width;
+    int plane_cap;           // rows of all planes together
+};
+
+// A tile's start and epilogue, in K blocks' time (measured: a dW tile of 1 block takes 4.4
+// blocks' time, one of 4 blocks 7.2).
+constexpr int kTileBlocks = 3;
+
+__host__ __device__ inline int ceil_int(int a, int b) { return (a + b - 1) / b; }
+
+// Time of the backward's products with about `splits` K splits of dx, in K blocks of a CTA pair
+// (infinity: not possible).  dx = G W has few tiles (rows x width) with a long K axis, a piece
+// of the vocabulary; dx and dW tiles share one launch, so it takes the mean over the pairs or
+// the rounds of dx tiles alone, whichever is longer, plus the fp32 planes' write and read at
+// 1.6 MB per block's time (0.33 us at 5 TB/s).
+__host__ __device__ inline float split_cost(const BackCosts &c, int rows, int splits, int &kb_per)
+{
+    kb_per = ceil_int(c.kbs, splits);
+    const int used = ceil_int(c.kbs, kb_per), plane_rows = ceil_int(rows, 32) * 32;
+    if ((splits > 1 && kb_per < 4) || static_cast<int64_t>(used) * plane_rows > c.plane_cap)
+        return INFINITY;
+    const float dx_tiles = static_cast<float>(ceil_int(rows, 2 * kBM)) * c.n_tiles * used;
+    const float dx_time = static_cast<float>(kb_per + kTileBlocks);
+    const float dw = static_cast<float>(c.dw_m_tiles) * c.n_tiles * (ceil_int(rows, kBK) + kTileBlocks);
+    const float mean = (dx_tiles * dx_time + dw) / c.units;
+    const float rounds = ceilf(dx_tiles / c.units) * dx_time;
+    return fmaxf(mean, rounds) * c.pieces + static_cast<float>(used) * rows * c.width * (8.0f / 1.6e6f);
+}
+
+// One warp: the shape with the least cost.
+__device__ __forceinline__ BackShape choose_shape(const BackCosts &c, int rows, int lane)
+{
+    float best = INFINITY;
+    int best_per = c.kbs;
+    for (int splits = 1 + lane; splits <= c.units; splits += 32) {
+        int per;
+        const float cost = split_cost(c, rows, splits, per);
+        if (cost < best) {
+            best = cost;
+            best_per = per;
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, best, o);
+        const int other_per = __shfl_xor_sync(0xffffffffu, best_per, o);
+        if (other < best || (other == best && other_per > best_per)) {
+            best = other;
+            best_per = other_per;
+        }
+    }
+    return BackShape{rows, best_per, ceil_int(c.kbs, best_per), ceil_int(rows, 32) * 32};
+}
+
 constexpr uint32_t kAMnMajor = 1u << 15, kBMnMajor = 1u << 16; // instruction descriptor bits
 
 struct Params {
     int rows;                    // token rows (the most there can be)
-    const int *rows_used;        // how many of them there are, on the device (null: all)
+    const BackShape *shape;      // kGrad and kBack: how many of them there are, and dx's splits
     int n, n_tiles;              // output columns: the vocabulary's (kStats, kGrad), x's width (kBack)
     int bn;                      // tile width
     int num_kb;                  // kStats, kGrad: K blocks (of x's width)
@@ -119,7 +186,7 @@ struct Params {
     const float *row_lse2, *row_gain; // kGrad: lse log2(e), and g T s
     // kBack
     int vocab;                   // the piece's vocabulary columns: K of dx, rows of dW
-    int dx_splits, dx_kb_per;    // K splits of dx (0: no dx) and their K blocks
+    int want_dx;
     int dw_tiles;                // tiles of dW (0: no dW)
     int accumulate;              // add to the fp32 planes
     const float *inv_gain;       // 1 / s
@@ -214,10 +281,10 @@ __device__ __forceinline__ int64_t load_label(const void *labels, int bytes, int
                       : static_cast<int64_t>(static_cast<const int32_t *>(labels)[row]);
 }
 
-__device__ __forceinline__ void tma_store_add_3d(const CUtensorMap *map, uint32_t src, int32_t x, int32_t y, int32_t z)
+__device__ __forceinline__ void tma_store_add_2d(const CUtensorMap *map, uint32_t src, int32_t x, int32_t y)
 {
-    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(y), "r"(z)
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(y)
                  : "memory");
 }
 
@@ -272,7 +339,7 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
         }
         mbar_init(bar_drain, 1);
         fence_barrier_init();
-        if (MODE != kBack || p.dx_splits > 0) {
+        if (MODE != kBack || p.want_dx) {
             prefetch_tensor_map(&tm_a);
             prefetch_tensor_map(&tm_b);
             if (MODE != kStats)
@@ -306,7 +373,10 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
 
-    const int rows = p.rows_used ? *p.rows_used : p.rows;
+    BackShape shape{p.rows, 1, 0, 0};
+    if (MODE != kStats)
+        shape = *p.shape;
+    const int rows = shape.rows;
     struct Tile {
         int m0, n0, kb0, kbn, split;
         bool dw;
@@ -317,13 +387,14 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
     const int m_tiles = (rows + C::kTileM - 1) / C::kTileM;
     // kBack: the dx tiles (long: K is the piece of the vocabulary) are dealt out first, the dW
     // tiles (K: the rows) after them.  Where a last round of dx tiles leaves units without one,
-    // those take as many dW tiles more as fit into its time (in K blocks, a tile's start and
-    // epilogue counted as six); from then on every unit is level again.
-    const int dx_tiles = MODE == kBack ? p.dx_splits * m_tiles * p.n_tiles : 0;
+    // those take as many dW tiles more as fit into its time; from then on every unit is level
+    // again.
+    const int dx_kbs = (p.vocab + kBK - 1) / kBK; // a last piece has fewer, and fewer splits
+    const int dx_tiles = MODE == kBack && p.want_dx ? ceil_int(dx_kbs, shape.kb_per) * m_tiles * p.n_tiles : 0;
     const int dx_left = dx_tiles % units;
     const int dx_mine = dx_tiles / units + (unit < dx_left ? 1 : 0);
     const int dw_kbs = (rows + kBK - 1) / kBK;
-    const int dw_extra = dx_left > 0 ? (p.dx_kb_per + 6) / (dw_kbs + 6) : 0;
+    const int dw_extra = dx_left > 0 ? (shape.kb_per + kTileBlocks) / (dw_kbs + kTileBlocks) : 0;
     auto tile_at = [&](int i, Tile &tile) {
         tile.split = 0;
         tile.dw = false;
@@ -345,8 +416,8 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
             const int r = t - tile.split * per_split;
             tile.m0 = (r / p.n_tiles) * C::kTileM + static_cast<int>(rank) * kBM;
             tile.n0 = (r % p.n_tiles) * p.bn;
-            tile.kb0 = tile.split * p.dx_kb_per;
-            tile.kbn = min(p.dx_kb_per, (p.vocab + kBK - 1) / kBK - tile.kb0);
+            tile.kb0 = tile.split * shape.kb_per;
+            tile.kbn = min(shape.kb_per, dx_kbs - tile.kb0);
             return true;
         }
         const int j = i - dx_mine;
@@ -661,10 +732,11 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
                         filled();
                         if (lane == 0) {
                             if (c0 + 16 * hf < p.n) {
+                                const int plane_row = tile.split * shape.plane_rows + row0;
                                 if (p.accumulate)
-                                    tma_store_add_3d(&tm_out, staging_s + buffer, c0 + 16 * hf, row0, tile.split);
+                                    tma_store_add_2d(&tm_out, staging_s + buffer, c0 + 16 * hf, plane_row);
                                 else
-                                    tma_store_3d(&tm_out, staging_s + buffer, c0 + 16 * hf, row0, tile.split);
+                                    tma_store_2d(&tm_out, staging_s + buffer, c0 + 16 * hf, plane_row);
                             }
                             bulk_commit_group();
                         }
@@ -904,7 +976,9 @@ struct Prepare {
     void *x_used;
     const float *lse, *grad;
     float *row_lse2, *row_gain, *inv_gain;
-    int *rows_used, *row_at; // labels: how many rows have a target, and where each went (-1: nowhere)
+    int *row_at; // labels: where each row went (-1: it has no target)
+    BackCosts costs;
+    BackShape *shape;
 };
 
 // s = 2^(13 - exponent of max |g T|) puts |g T s| in [2^13, 2^14): with |p - t| <= 1, G then
@@ -967,8 +1041,11 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
         total += warp_total[i];
     }
     const float s = common_gain(top * p.temperature, p.inv_gain);
-    if (blockIdx.x == 0 && threadIdx.x == 0)
-        *p.rows_used = max(total, 1); // a row of zeros where no row has a target
+    if (blockIdx.x == 0 && warp == 0) {
+        const BackShape shape = choose_shape(p.costs, max(total, 1), lane); // a row of zeros where none has a target
+        if (lane == 0)
+            *p.shape = shape;
+    }
 
     const int vectors = p.width / 8;
     const uint4 *x = static_cast<const uint4 *>(p.x);
@@ -1050,6 +1127,11 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
     for (int i = 0; i < kPrepWarps; ++i)
         top = fmaxf(top, warp_max[i]);
     const float s = common_gain(top * p.temperature, p.inv_gain);
+    if (blockIdx.x == 0 && warp == 0) {
+        const BackShape shape = choose_shape(p.costs, p.t.rows, lane);
+        if (lane == 0)
+            *p.shape = shape;
+    }
 
     const int vectors = p.width / 8;
     for (int row = blockIdx.x * kPrepWarps + warp; row < p.t.rows; row += gridDim.x * kPrepWarps) {
@@ -1269,14 +1351,15 @@ __global__ void __launch_bounds__(32 * kCombineRowWarps) combine_rows_kernel(con
 // from where they went, rows without a target are zero.  Eight elements per thread; blocks own
 // runs of kRows rows, and kRows rows of kPlanes planes are in flight together.
 template <bool kBf16, int kRows, int kPlanes>
-__global__ void __launch_bounds__(256) planes_kernel(const float *planes, int count, int rows, int width,
+__global__ void __launch_bounds__(256) planes_kernel(const float *planes, const BackShape *shape, int rows, int width,
                                                      const int *row_at, const float *inv_gain, uint4 *dx)
 {
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
     const float inv = *inv_gain;
     const int vectors = width / 8;
-    const size_t plane = static_cast<size_t>(rows) * vectors; // in pairs of float4
+    const int count = shape->splits;
+    const size_t plane = static_cast<size_t>(shape->plane_rows) * vectors; // in pairs of float4
     const float4 *all = reinterpret_cast<const float4 *>(planes);
     for (int row0 = blockIdx.x * kRows; row0 < rows; row0 += gridDim.x * kRows) {
         int from[kRows];
@@ -1431,43 +1514,15 @@ struct BackwardPlan {
     int64_t piece, pieces;   // vocabulary columns per piece of G
     int64_t ldg;             // elements per row of a piece
     int grad_bn, width_bn;   // tile widths over a piece's columns, and over x's width
-    int64_t splits;          // K splits of dx
+    BackCosts costs;
+    int64_t splits;          // K splits of dx if every row has a target
     float *row_lse2, *row_gain, *inv_gain, *t_prob, *dx_planes;
     int32_t *t_index;
-    int *rows_used, *row_at;
+    BackShape *shape;
+    int *row_at;
     void *x_used, *g;
     int64_t bytes;
 };
-
-// K splits of dx = G W, whose tiles (rows x width) are few while its K axis, a piece of the
-// vocabulary, is long: the count that finishes first, by K blocks of a CTA pair.  dx and dW
-// tiles share one launch, so its time is the mean over the pairs or the rounds of dx tiles
-// alone, whichever is longer (about six blocks for a tile's start and epilogue), plus the fp32
-// planes' write and read at 1.6 MB per block's time (0.33 us at 5 TB/s).
-int64_t dx_splits(const VocabLossLaunch &L, const BackwardPlan &b)
-{
-    const int64_t units = sm_count() / 2;
-    const int64_t n_tiles = ceil_div(L.width, b.width_bn);
-    const int64_t dx_tiles = ceil_div(L.rows, 2 * kBM) * n_tiles;
-    const int64_t dw = L.dweight ? ceil_div(b.piece, 2 * kBM) * n_tiles * (ceil_div(L.rows, kBK) + 6) : 0;
-    const int64_t kbs = ceil_div(b.piece, kBK);
-    int64_t best = 1;
-    double best_cost = INFINITY;
-    for (int64_t s = 1; s <= units; ++s) {
-        const int64_t per = ceil_div(kbs, s);
-        if (s > 1 && per < 4)
-            break;
-        const int64_t used = ceil_div(kbs, per);
-        const double mean = static_cast<double>(dx_tiles * used * (per + 6) + dw) / units;
-        const double rounds = static_cast<double>(ceil_div(dx_tiles * used, units) * (per + 6));
-        const double cost = std::max(mean, rounds) * b.pieces + static_cast<double>(used) * L.rows * L.width * 8 / 1.6e6;
-        if (cost < best_cost) {
-            best_cost = cost;
-            best = used;
-        }
-    }
-    return best;
-}
 
 BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
 {
@@ -1482,19 +1537,40 @@ BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
     b.ldg = round_up(b.piece, 64);
     b.grad_bn = logits_width(L.rows, b.piece, L.width, b.single, 32);
     b.width_bn = even_width(L.width);
-    b.splits = L.dx ? dx_splits(L, b) : 0;
+    b.costs.kbs = static_cast<int>(ceil_div(b.piece, kBK));
+    b.costs.pieces = static_cast<int>(b.pieces);
+    b.costs.n_tiles = static_cast<int>(ceil_div(L.width, b.width_bn));
+    b.costs.dw_m_tiles = L.dweight ? static_cast<int>(ceil_div(b.piece, 2 * kBM)) : 0;
+    b.costs.units = sm_count() / 2;
+    b.costs.width = static_cast<int>(L.width);
+    b.costs.plane_cap = INT_MAX;
+    float least = INFINITY;
+    int kb_per = 1;
+    for (int s = 1; s <= b.costs.units; ++s) {
+        const float cost = split_cost(b.costs, static_cast<int>(L.rows), s, kb_per);
+        if (cost < least) {
+            least = cost;
+            b.splits = ceil_div(b.costs.kbs, kb_per);
+        }
+    }
+    // Planes for those splits, or twice as many where that is at most 16 MB: fewer rows than
+    // there can be may want more of them.
+    const int64_t plane_rows = b.splits * round_up(L.rows, 32);
+    b.costs.plane_cap = static_cast<int>(
+        std::min<int64_t>(std::max(plane_rows, std::min(2 * plane_rows, (int64_t{16} << 20) / (4 * L.width))), INT_MAX));
     b.row_lse2 = arena.take<float>(L.rows);
     b.row_gain = arena.take<float>(L.rows);
     b.inv_gain = arena.take<float>(1);
     b.t_index = arena.take<int32_t>(L.rows * b.targets);
     b.t_prob = arena.take<float>(L.rows * b.targets);
     if (L.targets == 0) {
-        b.rows_used = arena.take<int>(1);
         b.row_at = arena.take<int>(L.rows);
     }
+    b.shape = arena.take<BackShape>(1);
     b.x_used = arena.take<uint16_t>(L.rows * L.width);
     b.g = arena.take<uint16_t>(L.rows * b.ldg);
-    b.dx_planes = arena.take<float>(b.splits * L.rows * L.width);
+    if (L.dx)
+        b.dx_planes = arena.take<float>(b.costs.plane_cap * L.width);
     b.bytes = arena.used;
     return b;
 }
@@ -1654,28 +1730,26 @@ cudaError_t launch_back(const VocabLossLaunch &L, const BackwardPlan &b, int64_t
     CUtensorMap maps[6] = {};
     Params p{};
     p.rows = static_cast<int>(L.rows);
-    p.rows_used = b.rows_used;
+    p.shape = b.shape;
     p.n = static_cast<int>(L.width);
     p.bn = b.width_bn;
     p.n_tiles = static_cast<int>(ceil_div(L.width, b.width_bn));
     p.vocab = static_cast<int>(cols);
     p.inv_gain = b.inv_gain;
     p.accumulate = col0 > 0 ? 1 : 0;
-    p.dx_kb_per = 1;
     int64_t tiles = 0;
     if (L.dx) {
         const uint16_t *w = static_cast<const uint16_t *>(L.weight) + col0 * L.width;
-        const int64_t dims[3] = {L.width, L.rows, b.splits};
-        const int64_t strides[2] = {L.width * 4, L.rows * L.width * 4};
-        const uint32_t box[3] = {16u, 32u, 1u};
+        const int64_t dims[2] = {L.width, b.costs.plane_cap};
+        const int64_t strides[1] = {L.width * 4};
+        const uint32_t box[2] = {16u, 32u};
         if (!operand_map(&maps[0], kBf16, false, b.g, L.rows, cols, b.ldg, tile_rows(L.rows)) ||
             !operand_map(&maps[1], kBf16, true, w, cols, L.width, L.width, 0) ||
-            !make_map_nd(&maps[2], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, b.dx_planes, dims, strides, box,
+            !make_map_nd(&maps[2], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, b.dx_planes, dims, strides, box,
                          CU_TENSOR_MAP_SWIZZLE_64B))
             return cudaErrorInvalidValue;
-        p.dx_kb_per = static_cast<int>(ceil_div(ceil_div(b.piece, kBK), b.splits));
-        p.dx_splits = static_cast<int>(ceil_div(ceil_div(cols, kBK), p.dx_kb_per)); // a last piece has fewer
-        tiles += p.dx_splits * ceil_div(L.rows, 2 * kBM) * p.n_tiles;
+        p.want_dx = 1;
+        tiles += 2 * b.splits * ceil_div(L.rows, 2 * kBM) * p.n_tiles;
     }
     if (L.dweight) {
         uint16_t *dw = static_cast<uint16_t *>(L.dweight) + col0 * L.width;
@@ -1715,8 +1789,9 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
     q.row_lse2 = b.row_lse2;
     q.row_gain = b.row_gain;
     q.inv_gain = b.inv_gain;
-    q.rows_used = b.rows_used;
     q.row_at = b.row_at;
+    q.costs = b.costs;
+    q.shape = b.shape;
     cudaError_t err;
     if (L.targets > 0) {
         const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, kPrepWarps), 4 * sm_count());
@@ -1737,7 +1812,7 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
         if (!map16(&out, kBf16, b.g, L.rows, cols, b.ldg, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B))
             return cudaErrorInvalidValue;
         Params p{};
-        p.rows_used = b.rows_used;
+        p.shape = b.shape;
         p.t_index = b.t_index;
         p.t_prob = b.t_prob;
         p.targets = b.targets;
@@ -1756,7 +1831,7 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
         const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, few ? 4 : 1), 4096 / threads * sm_count());
         const auto kernel = few ? planes_kernel<kBf16, 4, 1> : planes_kernel<kBf16, 1, 8>;
         err = launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(static_cast<unsigned>(threads)), stream,
-                         static_cast<const float *>(b.dx_planes), static_cast<int>(b.splits),
+                         static_cast<const float *>(b.dx_planes), static_cast<const BackShape *>(b.shape),
                          static_cast<int>(L.rows), static_cast<int>(L.width), static_cast<const int *>(b.row_at),
                          static_cast<const float *>(b.inv_gain), static_cast<uint4 *>(L.dx));
     }
