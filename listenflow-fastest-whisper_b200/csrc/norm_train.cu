@@ -570,8 +570,7 @@ using namespace tnorm;
 int group_threads(int64_t cols) { return static_cast<int>((cols / 8 + 31) / 32 * 32); }
 int group_count(int64_t cols) { return std::min(kMaxGroups, std::max(1, kMaxThreads / group_threads(cols))); }
 
-// Rows per step: several once every group of the GPU has that many, else one, which spreads
-// few rows over the most groups.
+// Blocks that share the rows, at most one per SM.
 int grid_blocks(int64_t rows, int64_t cols, int rows_per_step)
 {
     const int64_t per_block = static_cast<int64_t>(group_count(cols)) * rows_per_step;
@@ -581,17 +580,21 @@ int grid_blocks(int64_t rows, int64_t cols, int rows_per_step)
 constexpr int kForwardRows = 2, kBackwardRows = 2;
 constexpr int kRingBytes = 200 * 1024; // a block's rings
 
+// Rings and several rows per step once every group of the GPU has that many rows, else one row
+// per step, which spreads few rows over the most groups.  Forward of 512 x 1280: 2.7 us without
+// rings, 3.3 with; 1184 x 1280: 4.1 and 3.5; 4000 x 1280: 11.0 and 8.3.
 bool many_rows(int64_t rows, int64_t cols, int rows_per_step)
 {
     return rows >= static_cast<int64_t>(sm_count()) * group_count(cols) * rows_per_step;
 }
 
-// Rows that one cluster of eight blocks handles in at most four steps of its groups, as fast
-// as the whole GPU and a second launch would (20 x 1280: 4.2 + 2.1 us and the launch against
-// one of 5 us).
+// Rows that one cluster of eight blocks handles in at most three steps of its groups.  It needs
+// one launch and no workspace, some 4 us of a caller's time, and on the GPU takes as long as
+// two launches over all SMs for one step (64 x 1280: 6.8 us against 6.2) and 2 to 4 us longer
+// for three (128 x 1280: 8.2 against 5.8; at 256 rows it would be 11.5 against 6.2).
 bool one_cluster(int64_t rows, int64_t cols)
 {
-    return rows <= 4 * int64_t{kClusterBlocks} * group_count(cols) * kBackwardRows;
+    return rows <= 3 * int64_t{kClusterBlocks} * group_count(cols) * kBackwardRows;
 }
 
 int backward_blocks(int64_t rows, int64_t cols)

@@ -1413,14 +1413,17 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Up to this many rows one CTA computes a tile instead of a pair: the rows fit one
-// accumulator and W is streamed once.
+// accumulator and W is streamed once.  128 x 1280 x 51866: forward 29.6 us and backward 92 us,
+// with pairs 30.7 and 94.
 constexpr int64_t kSingleRows = 128;
 
-// Up to this many rows the forward's last step takes a warp per row (20 rows: 10 us with 32
-// rows per block, 4.9 us with a warp each); above, its strided reads cost more than they save.
+// Up to this many rows the forward's last step takes a warp per row; above, its strided reads
+// cost more than they save.  Whole forward over 384: 333 rows 22.2 us with a warp per row, 25.8
+// with 32 rows per block; 1024 rows 35.8 and 37.1; 2048 rows 71.5 and 66.0.
 constexpr int64_t kCombineRows = 1024;
 
-// Bytes of one piece of G.
+// Bytes of one piece of G: the memory a step may take for it, whatever its rows.  Larger pieces
+// are faster (14336 x 1280 x 51866: 6.07 ms with 256 MB, 5.94 with 512, 5.82 with all of G).
 constexpr int64_t kPieceBytes = int64_t{512} << 20;
 
 // Calls f with the entries per lane (1, 2, 4 or 8) that hold `targets` entries in a warp.
@@ -1825,7 +1828,8 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
             return err;
     }
     if (L.dx) {
-        // Few planes: four rows at a time; many (few rows): eight planes of one.
+        // Few planes: four rows at a time (14336 x 1280, one plane: 20 us, with eight planes of one
+        // row 60); many, which means few rows: eight planes of one.
         const bool few = b.splits <= 2;
         const int64_t threads = std::min<int64_t>(round_up(L.width / 8, 32), 256);
         const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, few ? 4 : 1), 4096 / threads * sm_count());
