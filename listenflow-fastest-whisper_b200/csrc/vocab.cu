@@ -16,7 +16,7 @@
 //            transposed times x (its rows of dW), one list of tiles shared out over the SMs
 // A piece of G is the only n x (part of V) tensor that ever exists.
 //
-// Rows without a target are left out of the gradients' products altogether (labels).
+// Rows without a target are left out of the gradients' products altogether.
 //
 // The work is bound by the tensor cores (2 n V d flops per product, four products in a training
 // step: the logits are formed twice because they are not kept) once n exceeds a few hundred
@@ -873,10 +873,10 @@ __device__ __forceinline__ void sort_keys(uint32_t (&key)[R], int lane)
 // order, the rest INT_MAX.  A sort key is the column with the entry's number below it (22 + 8
 // bits), so equal tokens keep their order.  Returns whether the row has any, with (negative
 // entropy, sum) of its probabilities in 64 bits: the loss is a difference of terms near
-// log(V), so it is formed from unrounded ones.
+// log(V), so it is formed from unrounded ones.  probs, keys: scratch of 32 R.
 template <int R>
-__device__ __forceinline__ bool sort_targets(const Targets &t, int row, int lane, float *probs, double &entropy,
-                                             double &total)
+__device__ __forceinline__ bool sort_targets(const Targets &t, int row, int lane, float *probs, uint32_t *keys,
+                                             double &entropy, double &total)
 {
     constexpr uint32_t kNone = 0xFFFFFFFFu;
     const size_t base = static_cast<size_t>(row) * t.count;
@@ -936,38 +936,59 @@ __device__ __forceinline__ bool sort_targets(const Targets &t, int row, int lane
     if (any)
         entropy -= total * log(static_cast<double>(sum));
     sort_keys<R>(key, lane);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        keys[lane + 32 * i] = key[i];
     __syncwarp();
+    // A token that occurs several times has their sum at its first entry and 0 at the others, so
+    // that dz subtracts it once: many small subtractions from a probability would each round.
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int j = lane + 32 * i;
         if (j < t.count) {
-            t.index[base + j] = key[i] == kNone ? INT_MAX : static_cast<int32_t>(key[i] >> 8);
-            t.prob[base + j] = key[i] == kNone ? 0.0f : probs[key[i] & 255u];
+            const uint32_t col = key[i] >> 8;
+            float prob = key[i] == kNone ? 0.0f : probs[key[i] & 255u];
+            if (key[i] != kNone && j > 0 && keys[j - 1] >> 8 == col) {
+                prob = 0.0f;
+            } else if (key[i] != kNone && j + 1 < t.count && keys[j + 1] >> 8 == col) {
+                double sum_of_equals = prob;
+                for (int o = j + 1; o < t.count && keys[o] >> 8 == col; ++o)
+                    sum_of_equals += probs[keys[o] & 255u];
+                prob = static_cast<float>(sum_of_equals);
+            }
+            t.index[base + j] = key[i] == kNone ? INT_MAX : static_cast<int32_t>(col);
+            t.prob[base + j] = prob;
         }
     }
     __syncwarp();
     return any;
 }
 
-// Forward of the distillation: sorted targets, and (entropy, sum) per row.
+// Sorted targets; in the forward (entropy, sum) per row, in the backward whether the row has any
+// target (0, else -1).
 template <int R>
-__global__ void __launch_bounds__(32 * kPrepWarps) targets_kernel(const Targets t, double2 *row_terms)
+__global__ void __launch_bounds__(32 * kPrepWarps) targets_kernel(const Targets t, double2 *row_terms, int32_t *marks)
 {
     __shared__ float probs[kPrepWarps][32 * R];
+    __shared__ uint32_t keys[kPrepWarps][32 * R];
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     for (int row = blockIdx.x * kPrepWarps + warp; row < t.rows; row += gridDim.x * kPrepWarps) {
         double entropy, total;
-        sort_targets<R>(t, row, lane, probs[warp], entropy, total);
-        if (lane == 0)
+        const bool any = sort_targets<R>(t, row, lane, probs[warp], keys[warp], entropy, total);
+        if (lane == 0 && row_terms)
             row_terms[row] = make_double2(entropy, total);
+        if (lane == 0 && marks)
+            marks[row] = any ? 0 : -1;
     }
 }
 
 struct Prepare {
-    Targets t;            // distillation (t.tokens set), or
-    const void *labels;   // one label per row
+    Targets t;            // the targets' place; a teacher's entries
+    const int32_t *sorted_index; // a teacher's sorted targets, row by row, before the rows move
+    const float *sorted_prob;
+    const void *labels;   // one label per row, or a teacher's marks (0, -1 to be ignored)
     int label_bytes;
     int64_t ignore_index;
     float temperature;
@@ -976,7 +997,7 @@ struct Prepare {
     void *x_used;
     const float *lse, *grad;
     float *row_lse2, *row_gain, *inv_gain;
-    int *row_at; // labels: where each row went (-1: it has no target)
+    int *row_at; // where each row went (-1: it has no target)
     BackCosts costs;
     BackShape *shape;
 };
@@ -993,13 +1014,14 @@ __device__ __forceinline__ float common_gain(float top, float *inv_gain)
 
 constexpr int kHeadVectors = 5; // 1280 elements of a row per lane group, requested ahead
 
-// Backward's first step with labels.  The rows that have a target move together, in order:
-// their states, labels, lse and gain g T s.  The others (padding, in a batch of transcripts)
+// Backward's first step.  The rows that have a target move together, in order: their states,
+// targets, lse and gain g T s.  The others (padding, in a batch of transcripts)
 // take no part in the products, so whatever they hold, NaN included, reaches nothing and costs
 // nothing.  Up to 255 zero rows follow, to the end of a tile, so that what a tile reads there
 // adds nothing.  Each block counts the valid labels before its rows itself (a few KB of reads),
 // which is why there is one large block per SM.
 constexpr int kRowWarps = 32;
+template <bool kTeacher>
 __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prepare p, int rows_per_block)
 {
     __shared__ float warp_max[kRowWarps];
@@ -1076,9 +1098,18 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
             for (int i = lane + 32 * kHeadVectors; i < vectors; i += 32)
                 dst[i] = src[i];
             const int64_t label = __shfl_sync(0xffffffffu, mine, j);
-            if (lane == 0) {
+            if (kTeacher) {
+                const size_t entries_from = static_cast<size_t>(row) * p.t.count;
+                const size_t entries_to = static_cast<size_t>(to) * p.t.count;
+                for (int i = lane; i < p.t.count; i += 32) {
+                    p.t.index[entries_to + i] = p.sorted_index[entries_from + i];
+                    p.t.prob[entries_to + i] = p.sorted_prob[entries_from + i];
+                }
+            } else if (lane == 0) {
                 p.t.index[to] = static_cast<int32_t>(label);
                 p.t.prob[to] = 1.0f;
+            }
+            if (lane == 0) {
                 p.row_lse2[to] = p.lse[row] * kLog2e;
                 p.row_gain[to] = p.grad[row] * p.temperature * s;
             }
@@ -1089,22 +1120,26 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
     for (int row = total + blockIdx.x * kRowWarps + warp; row < tail; row += gridDim.x * kRowWarps) {
         for (int i = lane; i < vectors; i += 32)
             x_used[static_cast<size_t>(row) * vectors + i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = lane; i < p.t.count; i += 32) {
+            p.t.index[static_cast<size_t>(row) * p.t.count + i] = INT_MAX;
+            p.t.prob[static_cast<size_t>(row) * p.t.count + i] = 0.0f;
+        }
         if (lane == 0) {
-            p.t.index[row] = INT_MAX;
-            p.t.prob[row] = 0.0f;
             p.row_lse2[row] = 0.0f;
             p.row_gain[row] = 0.0f;
         }
     }
 }
 
-// Backward's first step with a teacher: per row its sorted targets (up to 32 R), lse and gain,
+// The same with a teacher and few rows, none of which moves (a tile holds them all, so nothing
+// would be saved): per row its sorted targets (up to 32 R), lse and gain,
 // and a copy of x whose rows without a target are zero, so that whatever those hold, NaN
 // included, reaches neither G nor dW.
 template <int R>
 __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const Prepare p)
 {
     __shared__ float probs[kPrepWarps][32 * R];
+    __shared__ uint32_t keys[kPrepWarps][32 * R];
     __shared__ float warp_max[kPrepWarps];
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
@@ -1145,7 +1180,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
             if (lane + 32 * i < vectors)
                 head[i] = src[lane + 32 * i];
         double entropy, total;
-        const bool any = sort_targets<R>(p.t, row, lane, probs[warp], entropy, total);
+        const bool any = sort_targets<R>(p.t, row, lane, probs[warp], keys[warp], entropy, total);
         if (lane == 0) {
             p.row_lse2[row] = any ? p.lse[row] * kLog2e : 0.0f;
             p.row_gain[row] = any ? p.grad[row] * p.temperature * s : 0.0f;
@@ -1511,16 +1546,24 @@ ForwardPlan plan_forward(const VocabLossLaunch &L, void *workspace)
     return f;
 }
 
+// Up to this many rows a teacher's rows without an entry stay where they are: the others would
+// fill as many tiles without them, and moving them takes one more launch.  Above it padding costs
+// nothing.  Backward, 32 entries, 51866 tokens, moved / in place, us: 256 rows of 512 63 / 57, a
+// third of them padding 60 / 57; 300 rows 76 / 73, a third 62 / 72; 1024 rows 150 / 148, a
+// third 117 / 140; 2240 rows of 1280, a third 524-586 / 623.
+constexpr int64_t kTeacherMoveRows = 256;
+
 struct BackwardPlan {
     bool single;             // kGrad by one CTA per tile
+    bool moves;              // rows without a target are left out
     int targets;
     int64_t piece, pieces;   // vocabulary columns per piece of G
     int64_t ldg;             // elements per row of a piece
     int grad_bn, width_bn;   // tile widths over a piece's columns, and over x's width
     BackCosts costs;
     int64_t splits;          // K splits of dx if every row has a target
-    float *row_lse2, *row_gain, *inv_gain, *t_prob, *dx_planes;
-    int32_t *t_index;
+    float *row_lse2, *row_gain, *inv_gain, *t_prob, *sorted_prob, *dx_planes;
+    int32_t *t_index, *sorted_index, *marks;
     BackShape *shape;
     int *row_at;
     void *x_used, *g;
@@ -1532,6 +1575,7 @@ BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
     BackwardPlan b{};
     Arena arena{static_cast<uint8_t *>(workspace)};
     b.single = L.rows <= kSingleRows;
+    b.moves = L.targets == 0 || L.rows > kTeacherMoveRows;
     b.targets = L.targets > 0 ? L.targets : 1;
     const int64_t most = std::max<int64_t>(256, kPieceBytes / 2 / L.rows / 256 * 256);
     b.pieces = ceil_div(L.vocab, most);
@@ -1566,8 +1610,12 @@ BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
     b.inv_gain = arena.take<float>(1);
     b.t_index = arena.take<int32_t>(L.rows * b.targets);
     b.t_prob = arena.take<float>(L.rows * b.targets);
-    if (L.targets == 0) {
+    if (b.moves)
         b.row_at = arena.take<int>(L.rows);
+    if (b.moves && L.targets > 0) {
+        b.marks = arena.take<int32_t>(L.rows);
+        b.sorted_index = arena.take<int32_t>(L.rows * b.targets);
+        b.sorted_prob = arena.take<float>(L.rows * b.targets);
     }
     b.shape = arena.take<BackShape>(1);
     b.x_used = arena.take<uint16_t>(L.rows * L.width);
@@ -1683,7 +1731,7 @@ cudaError_t run_forward(const VocabLossLaunch &L, cudaStream_t stream)
         const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, kPrepWarps), 8 * sm_count());
         err = per_lane(L.targets, [&](auto r) {
             return launch_pdl(targets_kernel<decltype(r)::value>, dim3(static_cast<unsigned>(blocks)),
-                              dim3(32 * kPrepWarps), stream, t, f.row_terms);
+                              dim3(32 * kPrepWarps), stream, t, f.row_terms, static_cast<int32_t *>(nullptr));
         });
         if (err != cudaSuccess)
             return err;
@@ -1795,17 +1843,33 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
     q.row_at = b.row_at;
     q.costs = b.costs;
     q.shape = b.shape;
+    const dim3 teacher_grid(static_cast<unsigned>(std::min<int64_t>(ceil_div(L.rows, kPrepWarps), 8 * sm_count())));
+    const int64_t per_block = round_up(ceil_div(L.rows, sm_count()), kRowWarps);
+    const dim3 row_grid(static_cast<unsigned>(ceil_div(L.rows, per_block)));
     cudaError_t err;
-    if (L.targets > 0) {
-        const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, kPrepWarps), 4 * sm_count());
+    if (L.targets == 0) {
+        err = launch_pdl(prepare_rows_kernel<false>, row_grid, dim3(32 * kRowWarps), stream, q,
+                         static_cast<int>(per_block));
+    } else if (!b.moves) {
         err = per_lane(L.targets, [&](auto r) {
-            return launch_pdl(prepare_teacher_kernel<decltype(r)::value>, dim3(static_cast<unsigned>(blocks)),
-                              dim3(32 * kPrepWarps), stream, q);
+            return launch_pdl(prepare_teacher_kernel<decltype(r)::value>, teacher_grid, dim3(32 * kPrepWarps), stream, q);
         });
     } else {
-        const int64_t per_block = round_up(ceil_div(L.rows, sm_count()), kRowWarps);
-        err = launch_pdl(prepare_rows_kernel, dim3(static_cast<unsigned>(ceil_div(L.rows, per_block))),
-                         dim3(32 * kRowWarps), stream, q, static_cast<int>(per_block));
+        Targets t = q.t;
+        t.index = b.sorted_index;
+        t.prob = b.sorted_prob;
+        err = per_lane(L.targets, [&](auto r) {
+            return launch_pdl(targets_kernel<decltype(r)::value>, teacher_grid, dim3(32 * kPrepWarps), stream, t,
+                              static_cast<double2 *>(nullptr), b.marks);
+        });
+        q.sorted_index = b.sorted_index;
+        q.sorted_prob = b.sorted_prob;
+        q.labels = b.marks;
+        q.label_bytes = 4;
+        q.ignore_index = -1;
+        if (err == cudaSuccess)
+            err = launch_pdl(prepare_rows_kernel<true>, row_grid, dim3(32 * kRowWarps), stream, q,
+                             static_cast<int>(per_block));
     }
     if (err != cudaSuccess)
         return err;

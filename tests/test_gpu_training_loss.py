@@ -164,6 +164,51 @@ def test_counts_of_valid_rows(training, n, valid):
     assert ref.worst(dx, e_dx, b_dx) <= 1 and ref.worst(dw, e_dw, b_dw) <= 1
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,vocab,k", [(40, 1, 216), (300, 2, 256), (70, 5, 250), (280, 40, 64)])
+def test_tokens_that_occur_many_times(training, n, vocab, k, dtype):
+    """Few different tokens in many entries: their probabilities add up before they meet the
+    softmax (with one token in all, the gradient is that of 1 - 1)."""
+    g, x, w, dloss = operands(n, 64, vocab, dtype, seed=3)
+    tokens = torch.randint(vocab, (n, k), generator=g, device="cuda", dtype=torch.int32)
+    logits = torch.randn((n, k), generator=g, device="cuda") * 3
+    compare(lambda: training.distillation_forward(x, w, tokens, logits, temperature=0.5),
+            lambda lse: training.distillation_backward(x, w, tokens, logits, lse, dloss, temperature=0.5),
+            x, w, dloss, ref.teacher_targets(tokens, logits, vocab, 0.5), 0.5, k)
+
+
+@pytest.mark.parametrize("n,valid", [(700, 0), (700, 1), (700, 63), (700, 65), (700, 256), (700, 257), (700, 700),
+                                     (257, 200), (256, 100), (100, 0), (100, 33)])
+@pytest.mark.parametrize("k", [3, 40, 200])
+def test_counts_of_valid_rows_with_a_teacher(training, n, valid, k):
+    """The same with a teacher, whose rows move above 256 rows: entries left out of every row
+    somewhere, whole rows of them, NaN in the states and gradients of those."""
+    d, vocab, temperature = 72, 600, 1.5
+    g, x, w, dloss = operands(n, d, vocab, torch.float16, seed=k)
+    tokens = torch.randint(vocab, (n, k), generator=g, device="cuda", dtype=torch.int32)
+    tokens[torch.rand((n, k), generator=g, device="cuda") < 0.2] = -1
+    logits = (torch.randn((n, k), generator=g, device="cuda") * 3).half()
+    out = torch.ones(n, dtype=torch.bool, device="cuda")
+    out[torch.randperm(n, generator=g, device="cuda")[:valid]] = False
+    tokens[out] = -1
+    x[out], dloss[out] = float("nan"), float("nan")
+    losses, lse = training.distillation_forward(x, w, tokens, logits, temperature=temperature)
+    poison = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(8)]
+    del poison  # cached by the allocator: the workspace's memory starts as NaN
+    dx, dw = training.distillation_backward(x, w, tokens, logits, lse, dloss, temperature=temperature)
+    targets = ref.teacher_targets(tokens, logits, vocab, temperature)
+    out |= ~targets[1]  # and rows whose entries were all left out by chance
+    clean = torch.where(out.unsqueeze(1), 0.0, x).to(x.dtype)
+    e_loss, e_lse, grad = ref.vocab_loss(clean, w, targets, temperature)
+    b_loss, _ = ref.loss_bounds(clean, w, targets, e_loss, e_lse, temperature, k)
+    assert ref.worst(losses, e_loss, b_loss) <= 1 and not losses[out].any() and not dx[out].any()
+    dloss = torch.where(out, 0.0, dloss)
+    full = grad * dloss.double().unsqueeze(1)
+    e_dx, e_dw = full @ w.double(), full.t() @ clean.double()
+    b_dx, b_dw = ref.grad_bounds(clean, w, grad, dloss, e_lse, e_dx, e_dw, temperature)
+    assert ref.worst(dx, e_dx, b_dx) <= 1 and ref.worst(dw, e_dw, b_dw) <= 1
+
+
 def test_rows_without_teacher_entries(training):
     n, d, vocab, k = 40, 64, 500, 4
     g, x, w, dloss = operands(n, d, vocab, torch.float16)
