@@ -1144,23 +1144,51 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    // The largest finite |g|: every block reads all of them (a few KB).
-    float top = 0.0f;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < p.t.rows; i += 32 * kPrepWarps) {
-        const float g = fabsf(p.grad[i]);
-        top = fmaxf(top, g < INFINITY ? g : 0.0f);
+    // The largest finite |g| of the rows that have an entry: every block looks at all of them, a
+    // row per thread (there are kTeacherMoveRows at most).  A row's first entry says mostly
+    // that it has one; a row whose first is left out matters only if its |g| is larger than
+    // those, and its warp then reads the others.
+    auto is_entry = [&](size_t at) {
+        const int32_t token = p.t.tokens[at];
+        return token >= 0 && token < p.t.vocab && load_float(p.t.logits, p.t.logit_type, at) != -INFINITY;
+    };
+    auto block_max = [&](float v) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        if (lane == 0)
+            warp_max[warp] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPrepWarps; ++i)
+            v = fmaxf(v, warp_max[i]);
+        return v;
+    };
+    const int mine = threadIdx.x;
+    float g = 0.0f;
+    bool known = true;
+    if (mine < p.t.rows) {
+        g = fabsf(p.grad[mine]);
+        g = g < INFINITY ? g : 0.0f;
+        known = is_entry(static_cast<size_t>(mine) * p.t.count);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1)
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0)
-        warp_max[warp] = top;
-    __syncthreads();
-    top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPrepWarps; ++i)
-        top = fmaxf(top, warp_max[i]);
+    float top = block_max(known ? g : 0.0f);
+    const bool open = !known && g > top;
+    if (__syncthreads_or(open)) {
+        float more = top;
+        for (uint32_t rows = __ballot_sync(0xffffffffu, open); rows; rows &= rows - 1u) {
+            const int from = __ffs(rows) - 1;
+            const size_t base = static_cast<size_t>(warp * 32 + from) * p.t.count;
+            bool has = false;
+            for (int i = lane; i < p.t.count; i += 32)
+                has |= is_entry(base + i);
+            const float g_there = __shfl_sync(0xffffffffu, g, from);
+            if (__any_sync(0xffffffffu, has))
+                more = fmaxf(more, g_there);
+        }
+        top = block_max(more);
+    }
     const float s = common_gain(top * p.temperature, p.inv_gain);
     if (blockIdx.x == 0 && warp == 0) {
         const BackShape shape = choose_shape(p.costs, p.t.rows, lane);
@@ -1546,12 +1574,14 @@ ForwardPlan plan_forward(const VocabLossLaunch &L, void *workspace)
     return f;
 }
 
-// Up to this many rows a teacher's rows without an entry stay where they are: the others would
+// Up to this many rows (a row per thread of prepare_teacher_kernel) a teacher's rows without an
+// entry stay where they are: the others would
 // fill as many tiles without them, and moving them takes one more launch.  Above it padding costs
 // nothing.  Backward, 32 entries, 51866 tokens, moved / in place, us: 256 rows of 512 63 / 57, a
 // third of them padding 60 / 57; 300 rows 76 / 73, a third 62 / 72; 1024 rows 150 / 148, a
 // third 117 / 140; 2240 rows of 1280, a third 524-586 / 623.
 constexpr int64_t kTeacherMoveRows = 256;
+static_assert(kTeacherMoveRows == 32 * kPrepWarps, "prepare_teacher_kernel: a row per thread");
 
 struct BackwardPlan {
     bool single;             // kGrad by one CTA per tile

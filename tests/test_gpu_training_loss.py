@@ -137,6 +137,30 @@ def test_ignored_rows_reach_nothing(training, n, dtype):
     assert not dx[out].any() and torch.equal(dx, dx_b) and torch.equal(dw, dw_b)
 
 
+@pytest.mark.parametrize("teacher", [False, True])
+@pytest.mark.parametrize("n", [60, 500])
+def test_large_gradients_of_ignored_rows(training, n, teacher):
+    """A finite but huge loss gradient at a row without a target scales nothing: neither fp16's
+    range nor its precision is spent on it."""
+    d, vocab, k = 128, 900, 40
+    g, x, w, dloss = operands(n, d, vocab, torch.float16)
+    labels = torch.randint(vocab, (n,), generator=g, device="cuda")
+    tokens = torch.randint(vocab, (n, k), generator=g, device="cuda", dtype=torch.int32)
+    logits = torch.randn((n, k), generator=g, device="cuda")
+    logits[:, :33] = -torch.inf  # the entries that count come late
+    out = torch.rand(n, generator=g, device="cuda") < 0.4
+    labels[out], tokens[out] = -100, -1
+    huge = torch.where(out, 1e30, dloss)
+    if teacher:
+        losses, lse = training.distillation_forward(x, w, tokens, logits)
+        grads = [training.distillation_backward(x, w, tokens, logits, lse, g) for g in (dloss, huge)]
+    else:
+        losses, lse = training.cross_entropy_forward(x, w, labels)
+        grads = [training.cross_entropy_backward(x, w, labels, lse, g) for g in (dloss, huge)]
+    assert not losses[out].any() and not grads[0][0][out].any()
+    assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+
+
 @pytest.mark.parametrize("n,valid", [(700, 0), (700, 1), (700, 31), (700, 33), (700, 64), (700, 65), (700, 255),
                                      (700, 256), (700, 257), (700, 699), (100, 1), (100, 63), (100, 70), (300, 290)])
 def test_counts_of_valid_rows(training, n, valid):
