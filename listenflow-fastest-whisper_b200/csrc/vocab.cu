@@ -625,7 +625,8 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
                     gain = p.row_gain[row];
                 }
             }
-            float run_max = -INFINITY, run_sum = 0.0f, run_t = 0.0f;
+            // From the lowest finite value up, so that a logit of -infinity adds exp2(-infinity).
+            float run_max = -FLT_MAX, run_sum = 0.0f, run_t = 0.0f;
 
             const bool ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_full + 8 * a, acc_ph, kSiteEpilogueAccFull));
             if (!ok) {
@@ -786,7 +787,7 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
                         const float m = other[lane];
                         const float next_max = fmaxf(run_max, m);
                         run_sum = fmaf(run_sum, exp2_approx(run_max - next_max),
-                                       other[32 + lane] * (m == -INFINITY ? 0.0f : exp2_approx(m - next_max)));
+                                       other[32 + lane] * exp2_approx(m - next_max));
                         run_max = next_max;
                         run_t += other[64 + lane];
                     }
@@ -1298,7 +1299,8 @@ __device__ __forceinline__ void write_row(const Combine &p, int row, float mx, f
         const int64_t label = load_label(p.labels, p.label_bytes, row);
         if (label >= 0 && label < p.vocab) {
             const double formed = p.label_z[row];
-            lse -= exp(formed - lse) * (formed - label_z);
+            if (formed != label_z) // both may be infinite
+                lse -= exp(formed - lse) * (formed - label_z);
             if (label != p.ignore_index)
                 loss = lse - label_z;
         } else if (label != p.ignore_index) {

@@ -161,6 +161,33 @@ def test_large_gradients_of_ignored_rows(training, n, teacher):
     assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
 
 
+@pytest.mark.parametrize("n", [20, 300])
+@pytest.mark.parametrize("masked", [40, 300, 777])
+def test_logits_of_minus_infinity(training, n, masked):
+    """bf16 reaches products past fp32: columns whose logit is -infinity, a whole tile of them
+    too, count as probability 0, whatever their place; a label there has an infinite loss."""
+    d, vocab = 64, 1200
+    g, x, w, dloss = operands(n, d, vocab, torch.bfloat16)
+    x[:, 0], w[:, 0] = 0.0, 0.0
+    labels = torch.randint(masked, vocab, (n,), generator=g, device="cuda")
+    e_loss, e_lse, grad = ref.vocab_loss(x, w[masked:], ref.label_targets(labels - masked, vocab - masked, -100))
+    targets = ref.label_targets(labels - masked, vocab - masked, -100)
+    b_loss, b_lse = ref.loss_bounds(x, w[masked:], targets, e_loss, e_lse)
+    full = grad * dloss.double().unsqueeze(1)
+    e_dx, e_dw = full @ w[masked:].double(), full.t() @ x.double()
+    b_dx, b_dw = ref.grad_bounds(x, w[masked:], grad, dloss, e_lse, e_dx, e_dw)
+    big = x.clone()
+    big[:, 0], w[:masked, 0] = 1e20, -1e20
+    losses, lse = training.cross_entropy_forward(big, w, labels)
+    assert ref.worst(lse, e_lse, b_lse) <= 1 and ref.worst(losses, e_loss, b_loss) <= 1
+    dx, dw = training.cross_entropy_backward(big, w, labels, lse, dloss)
+    assert ref.worst(dx, e_dx, b_dx) <= 1 and ref.worst(dw[masked:, 1:], e_dw[:, 1:], b_dw[:, 1:]) <= 1
+    assert not dw[:masked].any()
+    labels[::2] = masked // 2
+    losses, lse_there = training.cross_entropy_forward(big, w, labels)
+    assert losses[::2].isposinf().all() and ref.worst(lse_there, e_lse, b_lse) <= 1
+
+
 @pytest.mark.parametrize("n,valid", [(700, 0), (700, 1), (700, 31), (700, 33), (700, 64), (700, 65), (700, 255),
                                      (700, 256), (700, 257), (700, 699), (100, 1), (100, 63), (100, 70), (300, 290)])
 def test_counts_of_valid_rows(training, n, valid):
