@@ -347,17 +347,24 @@ class Decoder:
 
     def final_states(self, transcripts: torch.Tensor, start_token: int = SOT,
                      ignore_index: int = training.IGNORE_INDEX) -> torch.Tensor:
-        """Teacher-forced decoding on the current stream: transcripts int32 [streams, length]
-        (length up to the cache's capacity and the position table) on the plan's device, padded with `ignore_index`.  Returns the
-        final states fp16 [length, streams, d] that predict each of their tokens: the state at
-        position t has read start_token and tokens 0 .. t - 1.  Leaves the caches holding the
-        transcripts' tokens but the last."""
+        """Teacher-forced decoding on the plan's device and its current stream: transcripts int32
+        [streams, length] there (length up to the cache's capacity and the position table),
+        padded with `ignore_index`.  Returns the final states fp16 [length, streams, d] that
+        predict each of their tokens: the state at position t has read start_token and tokens
+        0 .. t - 1.  Leaves the caches holding the transcripts' tokens but the last.  A token
+        outside the vocabulary sets fp8.decoder_error: what follows it in its transcript counts
+        for nothing."""
         c, s = self.config, self.streams
         if (transcripts.dtype != torch.int32 or transcripts.dim() != 2 or transcripts.shape[0] != s
                 or transcripts.device != self.tokens.device
                 or not 1 <= transcripts.shape[1] <= min(self.capacity, c.positions)):
             raise ValueError(f"transcripts must be int32 [{s}, 1 to {min(self.capacity, c.positions)}] on "
                              f"{self.tokens.device}")
+        with torch.cuda.device(self.tokens.device):
+            return self._final_states(transcripts, start_token, ignore_index)
+
+    def _final_states(self, transcripts: torch.Tensor, start_token: int, ignore_index: int) -> torch.Tensor:
+        c, s = self.config, self.streams
         length = transcripts.shape[1]
         # Padding is read as end of text; what it leads to is ignored by the losses.
         pad = min(EOT, c.vocab - 1)
@@ -392,7 +399,8 @@ class Decoder:
         length], 0 for padding, from a teacher's best logits [streams, length, k] (int32 tokens,
         fp16/bf16/fp32 logits): how far quantisation has moved a decoder from the one it was
         made of, token by token."""
-        if teacher_tokens.shape[:2] != transcripts.shape or teacher_logits.shape != teacher_tokens.shape:
+        if (teacher_tokens.dim() != 3 or teacher_tokens.shape[:2] != transcripts.shape
+                or teacher_logits.shape != teacher_tokens.shape):
             raise ValueError("teacher_tokens and teacher_logits must be [streams, length, k] like transcripts")
         states = self.final_states(transcripts, start_token, ignore_index)
         k = teacher_tokens.shape[2]

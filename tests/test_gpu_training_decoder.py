@@ -111,6 +111,27 @@ def test_refusals(plan, greedy):
                         torch.zeros((STREAMS, STEPS + 1, 2), device="cuda"))
 
 
+def test_refuses_teachers_of_other_ranks(plan, greedy):
+    tokens, _ = greedy
+    with pytest.raises(ValueError):
+        plan.divergence(tokens, tokens, torch.zeros_like(tokens, dtype=torch.float32))
+    with pytest.raises(ValueError):
+        plan.divergence(tokens, tokens.unsqueeze(2), torch.zeros((STREAMS, STEPS, 2), device="cuda"))
+
+
+def test_tokens_outside_the_vocabulary(plan, greedy, training, fp8):
+    """They are reported, cost nothing, and change neither what comes before them nor other streams."""
+    tokens, _ = greedy
+    losses = plan.score(tokens)
+    bad = tokens.clone()
+    bad[1, 2], bad[2, STEPS - 1] = plan.config.vocab, -5
+    got = plan.score(bad)
+    assert fp8.decoder_error() == 1 and training.token_error() == 1
+    assert got[1, 2] == 0 and got[2, STEPS - 1] == 0
+    assert torch.equal(got[0], losses[0]) and torch.equal(got[1, :2], losses[1, :2])
+    assert torch.equal(got[2, :-1], losses[2, :-1])
+
+
 def test_tuning_the_tail(plan, greedy, training):
     """The tail's parameters against the transcripts: the summed score's gradients by autograd
     agree with its change under a step, and the tuned parts are the decoder's own."""
