@@ -41,7 +41,7 @@ def compare(forward, backward, x, w, dloss, targets, temperature=1.0, entries=1)
     dx, dw = backward(lse)
     full = g * dloss.double().unsqueeze(1)
     e_dx, e_dw = full @ w.double(), full.t() @ x.double()
-    b_dx, b_dw = ref.grad_bounds(x, w, g, dloss, e_lse, e_dx, e_dw, temperature)
+    b_dx, b_dw = ref.grad_bounds(x, w, g, dloss, e_lse, e_dx, e_dw, temperature, targets[0], entries)
     assert ref.worst(dx, e_dx, b_dx) <= 1
     assert ref.worst(dw, e_dw, b_dw) <= 1
     return losses, lse, dx, dw
@@ -77,6 +77,23 @@ def test_distillation(training, n, d, vocab, k, temperature, dtype):
     compare(lambda: training.distillation_forward(x, w, tokens, logits, temperature=temperature),
             lambda lse: training.distillation_backward(x, w, tokens, logits, lse, dloss, temperature=temperature),
             x, w, dloss, ref.teacher_targets(tokens, logits, vocab, temperature), temperature, k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d,vocab", [(3, 65536, 40), (300, 8200, 1030), (20000, 8, 3), (40, 8, 300001),
+                                       (2000, 4096, 1)])
+def test_extreme_shapes(training, n, d, vocab, dtype):
+    g, x, w, dloss = operands(n, d, vocab, dtype, scale=d ** -0.5)
+    labels = torch.randint(vocab, (n,), generator=g, device="cuda")
+    labels[torch.rand(n, generator=g, device="cuda") < 0.2] = -100
+    compare(lambda: training.cross_entropy_forward(x, w, labels),
+            lambda lse: training.cross_entropy_backward(x, w, labels, lse, dloss),
+            x, w, dloss, ref.label_targets(labels, vocab, -100))
+    tokens = torch.randint(vocab, (n, 33), generator=g, device="cuda", dtype=torch.int32)
+    logits = torch.randn((n, 33), generator=g, device="cuda")
+    compare(lambda: training.distillation_forward(x, w, tokens, logits),
+            lambda lse: training.distillation_backward(x, w, tokens, logits, lse, dloss),
+            x, w, dloss, ref.teacher_targets(tokens, logits, vocab, 1.0), 1.0, 33)
 
 
 def test_pieces_and_splits(training):

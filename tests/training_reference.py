@@ -127,11 +127,18 @@ def loss_bounds(x, weight, targets, losses, lse, temperature=1.0, entries=1):
     return temperature ** 2 * off + 2 * U32 * losses.abs(), off_lse
 
 
-def grad_bounds(x, weight, g, dloss, lse, dx, dweight, temperature=1.0):
+def grad_bounds(x, weight, g, dloss, lse, dx, dweight, temperature=1.0, t=None, entries=1):
     """G's error is p times the error of its exponent (the logit's, the given lse's rounding,
     the exponential's 2^-22), plus half a step of its 16-bit type, plus what the common scale
     2^13..2^14 over max |dloss T| flushes (2^-38 of that maximum); dx and dweight are sums of
-    vocab or rows products of the tensor cores over it, rounded once."""
+    vocab or rows products of the tensor cores over it, rounded once.
+
+    With the targets t given, p is g / T + t itself, also where it exceeds a target.  A teacher's
+    probabilities are off by 64 u at most, those of equal tokens together: exponents at a
+    distance D below the largest take three roundings, 3 u D, and the mean of D under t is at
+    most log(256) < 5.6, in the entries and again in their sum (17 u each); the exponential
+    is off by 4 u in both; the sum has 8 + 5 adds, the quotient and the sum of equals one
+    rounding each: 17 + 17 + 8 + 13 + 2 = 57."""
     dtype = x.dtype
     eps = torch.finfo(dtype).eps
     gain = dloss.double().abs().unsqueeze(1)
@@ -140,8 +147,12 @@ def grad_bounds(x, weight, g, dloss, lse, dx, dweight, temperature=1.0):
     soft = torch.minimum(p, torch.full_like(p, temperature))
     # Tighter where there is no target: p is |g| itself.
     soft = torch.where(g >= 0, torch.minimum(soft, g.clamp(min=0) + torch.where(g > 0, 0.0, temperature)), soft)
+    target = 4 * U32 * temperature
+    if t is not None:
+        soft = (g + temperature * t).clamp(min=0)
+        target = temperature * (4 + 64 * (t > 0) * (entries > 1)) * U32
     big = (dloss.double().abs().max() * temperature) * 2.0 ** -38
-    off_g = gain * (soft * (torch.expm1(dz) + 2.0 ** -20) + 4 * U32 * temperature) + gain * g.abs() * (eps / 2) + big
+    off_g = gain * (soft * (torch.expm1(dz) + 2.0 ** -20) + target) + gain * g.abs() * (eps / 2) + big
     full = gain * g.abs()
     w, a = weight.double().abs(), x.double().abs()
     vocab, rows = weight.shape[0], x.shape[0]
