@@ -370,8 +370,13 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
     // Everything this grid reads (the weights too: an optimizer may just have written them)
     // and writes belongs to the previous kernel until it completes.  The next kernel may only
     // then start, so that its own early reads cannot pass that one either.
-    griddepcontrol_wait();
-    griddepcontrol_launch_dependents();
+    // kStats after targets_kernel: x and W are complete since that one was let past its wait, and
+    // only the epilogue reads its targets.
+    const bool late = MODE == kStats && p.t_index != nullptr;
+    if (!late || warp >= 2) {
+        griddepcontrol_wait();
+        griddepcontrol_launch_dependents();
+    }
 
     BackShape shape{p.rows, 1, 0, 0};
     if (MODE != kStats)
@@ -1265,6 +1270,8 @@ __device__ __forceinline__ float dot16(uint4 a, uint4 b, float acc)
 // The tensor cores truncate each of the width / 16 steps of a logit's sum, which shifts large
 // logits, the label's above all, by some 1e-6 of their value.  One dot product per row
 // replaces the label's logit where it enters: the loss and, by its probability, the lse.
+// Its operands are the call's inputs, complete since the kernel before this one was let past its
+// own wait, so it runs before this kernel's.
 template <bool kBf16>
 __device__ __forceinline__ float label_product(const Combine &p, int row, int lane)
 {
@@ -1366,10 +1373,15 @@ __global__ void __launch_bounds__(32 * kCombineGroups) combine_kernel(const Comb
     __shared__ float s_max[kCombineGroups][32], s_sum[kCombineGroups][32];
     __shared__ double s_t[kCombineGroups][32];
     __shared__ float s_label[32];
-    griddepcontrol_wait();
-    griddepcontrol_launch_dependents();
     const int group = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int row = blockIdx.x * 32 + lane;
+    for (int i = group; p.labels && i < 32 && blockIdx.x * 32 + i < p.rows; i += kCombineGroups) {
+        const float z = label_product<kBf16>(p, blockIdx.x * 32 + i, lane);
+        if (lane == 0)
+            s_label[i] = z;
+    }
+    griddepcontrol_wait();
+    griddepcontrol_launch_dependents();
     float mx = -INFINITY, sum = 0.0f;
     double target = 0.0;
     if (row < p.rows)
@@ -1377,11 +1389,6 @@ __global__ void __launch_bounds__(32 * kCombineGroups) combine_kernel(const Comb
     s_max[group][lane] = mx;
     s_sum[group][lane] = sum;
     s_t[group][lane] = target;
-    for (int i = group; p.labels && i < 32 && blockIdx.x * 32 + i < p.rows; i += kCombineGroups) {
-        const float z = label_product<kBf16>(p, blockIdx.x * 32 + i, lane);
-        if (lane == 0)
-            s_label[i] = z;
-    }
     __syncthreads();
     if (group != 0 || row >= p.rows)
         return;
@@ -1395,14 +1402,14 @@ constexpr int kCombineRowWarps = 4;
 template <bool kBf16>
 __global__ void __launch_bounds__(32 * kCombineRowWarps) combine_rows_kernel(const Combine p)
 {
+    const int row = blockIdx.x * kCombineRowWarps + threadIdx.x / 32, lane = threadIdx.x % 32;
+    const float label_z = p.labels && row < p.rows ? label_product<kBf16>(p, row, lane) : 0.0f;
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
-    const int row = blockIdx.x * kCombineRowWarps + threadIdx.x / 32, lane = threadIdx.x % 32;
     if (row >= p.rows)
         return;
     float mx = -INFINITY, sum = 0.0f;
     double target = 0.0;
-    const float label_z = p.labels ? label_product<kBf16>(p, row, lane) : 0.0f;
     merge_tiles(p, row, lane, 32, mx, sum, target);
 #pragma unroll
     for (int o = 16; o; o >>= 1)
@@ -1419,12 +1426,13 @@ template <bool kBf16, int kRows, int kPlanes>
 __global__ void __launch_bounds__(256) planes_kernel(const float *planes, const BackShape *shape, int rows, int width,
                                                      const int *row_at, const float *inv_gain, uint4 *dx)
 {
-    griddepcontrol_wait();
-    griddepcontrol_launch_dependents();
+    // From the backward's first kernel, which the one before this waited for.
     const float inv = *inv_gain;
     const int vectors = width / 8;
     const int count = shape->splits;
     const size_t plane = static_cast<size_t>(shape->plane_rows) * vectors; // in pairs of float4
+    griddepcontrol_wait();
+    griddepcontrol_launch_dependents();
     const float4 *all = reinterpret_cast<const float4 *>(planes);
     for (int row0 = blockIdx.x * kRows; row0 < rows; row0 += gridDim.x * kRows) {
         int from[kRows];
