@@ -484,8 +484,9 @@ LFFW_FP8_API lffw_status lffw_layer_norm_grad(const lffw_layer_norm_grad_args *a
  * lffw_vocab_loss_grad reads lse and dloss (fp32 [rows], the gradients of the losses)
  * and writes, in `dtype`, dx [rows, width] and/or dweight [vocab, width]:
  *   G = dloss T (exp(z / T - lse) - t),  dx = G weight,  dweight = G^T x
- * G is formed piece by piece over the vocabulary and held in 16 bits (scaled by a power of
- * two so that fp16 neither overflows nor loses small probabilities); sums are fp32.
+ * G is formed piece by piece over the vocabulary and held in 16 bits, scaled so that fp16
+ * neither overflows nor loses small probabilities; where at most 128 rows have a target, in
+ * twice 16 bits.  Sums are fp32.
  * workspace holds lffw_vocab_loss_workspace(args, 0 for the loss, 1 for the gradients)
  * bytes (-1 for invalid arguments; it depends on the current device, the shape, the number
  * of targets and, for the gradients, on which of dx and dweight are set, never on contents).

@@ -96,12 +96,23 @@ struct Cfg {
     static_assert((2 * kStages + 5) * 8 + 8 <= kBarBytes, "barrier area");
 };
 
+// Up to this many rows G is held in two parts, its rounding to 16 bits and what that leaves off,
+// as further rows from lo_row on (with x's rows once more): the products are then those of an
+// unrounded G.  With more rows the roundings of G average out to as much as dx and dW's own
+// (1.3 to 1.45 times the error of those alone, measured); with few, single large elements decide
+// (1.9 times at 7 rows of 5 teacher's entries), and both parts fit one row tile of dx.  Backward
+// over 51866 tokens with one part and with two: 7 x 512 40 and 42 us, 20 x 1280 83 and 87,
+// 128 x 1280 93 and 108.
+constexpr int kSplitRows = 128;
+
 // The backward's shape, decided on the device once the rows that have a target are counted.
 struct BackShape {
-    int rows;       // of G and x_used
+    int rows;       // that have a target
+    int lo_row;     // where the second part's rows start (0: there is none)
+    int all_rows;   // of G and x_used
     int kb_per;     // K blocks of one split of dx
     int splits;     // planes of dx
-    int plane_rows; // rows from one plane to the next: rows, rounded up to a store's 32
+    int plane_rows; // rows from one plane to the next: all_rows, rounded up to a store's 32
 };
 
 // What the choice of dx's splits depends on.
@@ -111,6 +122,7 @@ struct BackCosts {
     int units;               // CTA pairs
     int width;
     int plane_cap;           // rows of all planes together
+    int part_rows;           // what lo_row is a multiple of
 };
 
 // A tile's start and epilogue, in K blocks' time (measured: a dW tile of 1 block takes 4.4
@@ -118,6 +130,13 @@ struct BackCosts {
 constexpr int kTileBlocks = 3;
 
 __host__ __device__ inline int ceil_int(int a, int b) { return (a + b - 1) / b; }
+
+// lo_row for that many rows: whole stores of 32 rows, or (part_rows 8 or 16) a part of one, where a
+// call has no more.
+__host__ __device__ inline int second_part(int rows, int part_rows)
+{
+    return rows <= kSplitRows ? ceil_int(rows, part_rows) * part_rows : 0;
+}
 
 // Time of the backward's products with about `splits` K splits of dx, in K blocks of a CTA pair
 // (infinity: not possible).  dx = G W has few tiles (rows x width) with a long K axis, a piece
@@ -139,8 +158,9 @@ __host__ __device__ inline float split_cost(const BackCosts &c, int rows, int sp
 }
 
 // One warp: the shape with the least cost.
-__device__ __forceinline__ BackShape choose_shape(const BackCosts &c, int rows, int lane)
+__device__ __forceinline__ BackShape choose_shape(const BackCosts &c, int with_target, int lane)
 {
+    const int lo_row = second_part(with_target, c.part_rows), rows = lo_row + with_target;
     float best = INFINITY;
     int best_per = c.kbs;
     for (int splits = 1 + lane; splits <= c.units; splits += 32) {
@@ -160,13 +180,14 @@ __device__ __forceinline__ BackShape choose_shape(const BackCosts &c, int rows, 
             best_per = other_per;
         }
     }
-    return BackShape{rows, best_per, ceil_int(c.kbs, best_per), ceil_int(rows, 32) * 32};
+    return BackShape{with_target, lo_row, rows, best_per, ceil_int(c.kbs, best_per), ceil_int(rows, 32) * 32};
 }
 
 constexpr uint32_t kAMnMajor = 1u << 15, kBMnMajor = 1u << 16; // instruction descriptor bits
 
 struct Params {
-    int rows;                    // token rows (the most there can be)
+    int rows;                    // token rows (the most there can be; kBack: rows of G)
+    int g_rows;                  // kGrad: rows that G has room for
     const BackShape *shape;      // kGrad and kBack: how many of them there are, and dx's splits
     int n, n_tiles;              // output columns: the vocabulary's (kStats, kGrad), x's width (kBack)
     int bn;                      // tile width
@@ -215,6 +236,15 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16)
     else
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+
+__device__ __forceinline__ float2 unpack16(uint32_t v, bool bf16)
+{
+    if (bf16)
+        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+    __half2 h;
+    memcpy(&h, &v, 4);
+    return __half22float2(h);
 }
 
 // fp32 pair a * b + c, each lane rounded once.
@@ -378,10 +408,10 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
         griddepcontrol_launch_dependents();
     }
 
-    BackShape shape{p.rows, 1, 0, 0};
+    BackShape shape{p.rows, 0, p.rows, 1, 0, 0};
     if (MODE != kStats)
         shape = *p.shape;
-    const int rows = shape.rows;
+    const int rows = MODE == kBack ? shape.all_rows : shape.rows;
     struct Tile {
         int m0, n0, kb0, kbn, split;
         bool dw;
@@ -587,9 +617,10 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
             __syncwarp();
             return C::kBuffers > 1 ? (stores++ & 1u) * 2048u : 0u;
         };
-        auto put = [&](uint32_t buffer, int j, uint4 w) {
-            *reinterpret_cast<uint4 *>(staging + buffer + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) = w;
+        auto put_row = [&](uint32_t buffer, int r, int j, uint4 w) {
+            *reinterpret_cast<uint4 *>(staging + buffer + r * 64 + ((j ^ ((r >> 1) & 3)) * 16)) = w;
         };
+        auto put = [&](uint32_t buffer, int j, uint4 w) { put_row(buffer, lane, j, w); };
         auto filled = [&] {
             fence_proxy_async_smem();
             __syncwarp();
@@ -600,8 +631,9 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
             const uint32_t acc_ph = (n >> 1) & 1;
             // G is also written (as zeros) for the rows that fill up a K block of dW.
             const int row_limit = MODE == kBack && tile.dw ? p.vocab
-                                  : MODE == kGrad          ? min((rows + kBK - 1) / kBK * kBK, p.rows)
-                                                           : rows;
+                                  : MODE != kGrad          ? rows
+                                  : shape.lo_row > 0       ? shape.lo_row
+                                                           : min((rows + kBK - 1) / kBK * kBK, p.g_rows);
             const int row0 = tile.m0 + quarter * 32;
             const int row = row0 + lane;
             const int col0 = tile.n0 + col_begin;
@@ -704,6 +736,11 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
                 }
                 float f[32];
                 if (MODE == kGrad) {
+                    if (row0 + 32 > rows && row >= rows) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            v[i] = 0u; // whatever lay in the tile; times a gain of 0
+                    }
                     const float2 ref = make_float2(-lse2, -lse2);
                     const float2 sc = make_float2(p.scale2, p.scale2);
 #pragma unroll
@@ -754,17 +791,47 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
                     for (int i = 0; i < 32; ++i)
                         f[i] = __uint_as_float(v[i]) * inv_gain;
                 }
-                const uint32_t buffer = next_buffer();
+                auto put16 = [&](uint32_t buffer, int r) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    put(buffer, j,
-                        make_uint4(pack16(f[8 * j], f[8 * j + 1], kBf16), pack16(f[8 * j + 2], f[8 * j + 3], kBf16),
-                                   pack16(f[8 * j + 4], f[8 * j + 5], kBf16),
-                                   pack16(f[8 * j + 6], f[8 * j + 7], kBf16)));
-                filled();
-                if (lane == 0) {
-                    tma_store_2d(MODE == kBack ? &tm_out2 : &tm_out, staging_s + buffer, c0, row0);
-                    bulk_commit_group();
+                    for (int j = 0; j < 4; ++j)
+                        put_row(buffer, r, j,
+                                make_uint4(pack16(f[8 * j], f[8 * j + 1], kBf16), pack16(f[8 * j + 2], f[8 * j + 3], kBf16),
+                                           pack16(f[8 * j + 4], f[8 * j + 5], kBf16),
+                                           pack16(f[8 * j + 6], f[8 * j + 7], kBf16)));
+                };
+                auto store16 = [&](uint32_t buffer, int first_row) {
+                    filled();
+                    if (lane == 0) {
+                        tma_store_2d(MODE == kBack ? &tm_out2 : &tm_out, staging_s + buffer, c0, first_row);
+                        bulk_commit_group();
+                    }
+                };
+                auto keep_rest = [&] { // what the rounding to 16 bits leaves off
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 kept = unpack16(pack16(f[i], f[i + 1], kBf16), kBf16);
+                        f[i] -= kept.x;
+                        f[i + 1] -= kept.y;
+                    }
+                };
+                const uint32_t buffer = next_buffer();
+                if (MODE == kGrad && shape.lo_row > 0 && shape.lo_row < 32) {
+                    // Both parts in one store, which ends with them (G has no more rows).
+                    if (lane < shape.lo_row) {
+                        put16(buffer, lane);
+                        keep_rest();
+                        put16(buffer, shape.lo_row + lane);
+                    }
+                    store16(buffer, row0);
+                    continue;
+                }
+                put16(buffer, lane);
+                store16(buffer, row0);
+                if (MODE == kGrad && shape.lo_row > 0) {
+                    keep_rest();
+                    const uint32_t again = next_buffer();
+                    put16(again, lane);
+                    store16(again, shape.lo_row + row0);
                 }
             }
             if (subs == 0) {
@@ -999,6 +1066,7 @@ struct Prepare {
     int64_t ignore_index;
     float temperature;
     int width;            // elements per row of x, a multiple of 8
+    int g_rows;           // rows of x_used, and of G
     const void *x;
     void *x_used;
     const float *lse, *grad;
@@ -1008,14 +1076,51 @@ struct Prepare {
     BackShape *shape;
 };
 
-// s = 2^(13 - exponent of max |g T|) puts |g T s| in [2^13, 2^14): with |p - t| <= 1, G then
-// fits fp16 and keeps 11 bits down to p = 2^-28.  Returns s; thread 0 of block 0 keeps 1 / s.
-__device__ __forceinline__ float common_gain(float top, float *inv_gain)
+// A rounding is off by up to half a step of its value's binade, which is least, relative to the
+// value, just under a power of two.  Most of G's weight is in the targets' elements, near -g T, so
+// of four gains a quarter of an octave apart the one is taken that rounds the g with the
+// least squared error (loss gradients that are all alike then end up where steps are finest).
+constexpr int kShares = 4;
+__device__ __forceinline__ float gain_share(int i)
 {
-    const int exponent = top > 0.0f && top < INFINITY ? min(max(ilogbf(top), -100), 100) : 13;
+    return i == 0 ? 1.0f : i == 1 ? 1.18920712f : i == 2 ? 1.41421356f : 1.68179283f;
+}
+
+// Adds the squared step of g times each share.
+__device__ __forceinline__ void add_steps(float (&steps)[kShares], float g)
+{
+#pragma unroll
+    for (int k = 0; k < kShares; ++k) {
+        const float step = __uint_as_float(__float_as_uint(g * gain_share(k)) & 0x7F800000u);
+        steps[k] = fmaf(step, step, steps[k]);
+    }
+}
+
+// The share with the least error; sums past fp32's range, up or down, leave the choice open.
+__device__ __forceinline__ float best_share(const float (&steps)[kShares])
+{
+    float share = 1.0f, least = INFINITY;
+#pragma unroll
+    for (int k = 0; k < kShares; ++k) {
+        const float error = steps[k] * (1.0f / (gain_share(k) * gain_share(k)));
+        if (error < least) {
+            least = error;
+            share = gain_share(k);
+        }
+    }
+    return share;
+}
+
+// The common gain s, a share times a power of two, puts max |g T s| in [2^13, 2^14): with
+// |p - t| <= 1, G then fits fp16 and keeps 11 bits down to p = 2^-28.  Returns s; thread 0 of
+// block 0 keeps 1 / s, by which the products' fp32 results are multiplied.
+__device__ __forceinline__ float common_gain(float top, float share, float *inv_gain)
+{
+    const int exponent = top > 0.0f && top < INFINITY ? min(max(ilogbf(top * share), -100), 100) : 13;
+    const float s = ldexpf(share, 13 - exponent);
     if (blockIdx.x == 0 && threadIdx.x == 0)
-        *inv_gain = ldexpf(1.0f, exponent - 13);
-    return ldexpf(1.0f, 13 - exponent);
+        *inv_gain = 1.0f / s;
+    return s;
 }
 
 constexpr int kHeadVectors = 5; // 1280 elements of a row per lane group, requested ahead
@@ -1027,10 +1132,11 @@ constexpr int kHeadVectors = 5; // 1280 elements of a row per lane group, reques
 // adds nothing.  Each block counts the valid labels before its rows itself (a few KB of reads),
 // which is why there is one large block per SM.
 constexpr int kRowWarps = 32;
+static_assert(kRowWarps == 32, "a lane per warp in the second step of a block's sums");
 template <bool kTeacher>
 __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prepare p, int rows_per_block)
 {
-    __shared__ float warp_max[kRowWarps];
+    __shared__ float warp_max[kRowWarps], warp_steps[kShares][kRowWarps];
     __shared__ int warp_before[kRowWarps], warp_total[kRowWarps];
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
@@ -1039,38 +1145,51 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
     const int end = min(begin + rows_per_block, p.t.rows);
     auto valid = [&](int64_t label) { return label != p.ignore_index && label >= 0 && label < p.t.vocab; };
     float top = 0.0f;
+    float steps[kShares] = {}; // sums of squared steps of g times each share
     int before = 0, total = 0;
+    // The same sums in every block: over its warps, then in each warp over the warps' (a lane each).
+    auto reduce = [&] {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+            total += __shfl_xor_sync(0xffffffffu, total, o);
+#pragma unroll
+            for (int k = 0; k < kShares; ++k)
+                steps[k] += __shfl_xor_sync(0xffffffffu, steps[k], o);
+        }
+    };
 #pragma unroll 8
     for (int i = threadIdx.x; i < p.t.rows; i += 32 * kRowWarps) {
-        const float g = fabsf(p.grad[i]);
+        const float grad = fabsf(p.grad[i]);
         const bool used = valid(load_label(p.labels, p.label_bytes, i));
-        top = fmaxf(top, used && g < INFINITY ? g : 0.0f);
+        const float g = used && grad < INFINITY ? grad : 0.0f;
+        top = fmaxf(top, g);
         before += used && i < begin;
         total += used;
+        add_steps(steps, g);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-    }
+    reduce();
     if (lane == 0) {
         warp_max[warp] = top;
         warp_before[warp] = before;
         warp_total[warp] = total;
+#pragma unroll
+        for (int k = 0; k < kShares; ++k)
+            warp_steps[k][warp] = steps[k];
     }
     __syncthreads();
-    top = 0.0f;
-    before = total = 0;
+    top = warp_max[lane];
+    before = warp_before[lane];
+    total = warp_total[lane];
 #pragma unroll
-    for (int i = 0; i < kRowWarps; ++i) {
-        top = fmaxf(top, warp_max[i]);
-        before += warp_before[i];
-        total += warp_total[i];
-    }
-    const float s = common_gain(top * p.temperature, p.inv_gain);
+    for (int k = 0; k < kShares; ++k)
+        steps[k] = warp_steps[k][lane];
+    reduce();
+    const float s = common_gain(top * p.temperature, best_share(steps), p.inv_gain);
+    const int rows = max(total, 1), lo_row = second_part(rows, p.costs.part_rows); // a row of zeros where none has a target
     if (blockIdx.x == 0 && warp == 0) {
-        const BackShape shape = choose_shape(p.costs, max(total, 1), lane); // a row of zeros where none has a target
+        const BackShape shape = choose_shape(p.costs, rows, lane);
         if (lane == 0)
             *p.shape = shape;
     }
@@ -1097,12 +1216,14 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
             for (int i = 0; i < kHeadVectors; ++i)
                 if (lane + 32 * i < vectors)
                     head[i] = src[lane + 32 * i];
+            for (int part = 0; part <= (lo_row > 0); ++part, dst += static_cast<size_t>(lo_row) * vectors) {
 #pragma unroll
-            for (int i = 0; i < kHeadVectors; ++i)
-                if (lane + 32 * i < vectors)
-                    dst[lane + 32 * i] = head[i];
-            for (int i = lane + 32 * kHeadVectors; i < vectors; i += 32)
-                dst[i] = src[i];
+                for (int i = 0; i < kHeadVectors; ++i)
+                    if (lane + 32 * i < vectors)
+                        dst[lane + 32 * i] = head[i];
+                for (int i = lane + 32 * kHeadVectors; i < vectors; i += 32)
+                    dst[i] = src[i];
+            }
             const int64_t label = __shfl_sync(0xffffffffu, mine, j);
             if (kTeacher) {
                 const size_t entries_from = static_cast<size_t>(row) * p.t.count;
@@ -1122,10 +1243,13 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
         }
         before += __popc(mask);
     }
-    const int tail = min(max((total + 255) / 256, 1) * 256, p.t.rows);
+    const int tail = min((rows + 255) / 256 * 256, p.g_rows);
     for (int row = total + blockIdx.x * kRowWarps + warp; row < tail; row += gridDim.x * kRowWarps) {
-        for (int i = lane; i < vectors; i += 32)
-            x_used[static_cast<size_t>(row) * vectors + i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < lo_row || row >= lo_row + total)
+            for (int i = lane; i < vectors; i += 32)
+                x_used[static_cast<size_t>(row) * vectors + i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row >= p.t.rows)
+            continue;
         for (int i = lane; i < p.t.count; i += 32) {
             p.t.index[static_cast<size_t>(row) * p.t.count + i] = INT_MAX;
             p.t.prob[static_cast<size_t>(row) * p.t.count + i] = 0.0f;
@@ -1146,7 +1270,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
 {
     __shared__ float probs[kPrepWarps][32 * R];
     __shared__ uint32_t keys[kPrepWarps][32 * R];
-    __shared__ float warp_max[kPrepWarps];
+    __shared__ float warp_max[kPrepWarps], warp_steps[kPrepWarps][kShares];
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -1195,7 +1319,30 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
         }
         top = block_max(more);
     }
-    const float s = common_gain(top * p.temperature, p.inv_gain);
+    const int lo_row = second_part(p.t.rows, p.costs.part_rows);
+    float share = 1.0f;
+    if (lo_row == 0) { // the rows known to have an entry decide
+        float steps[kShares] = {};
+        add_steps(steps, known ? g : 0.0f);
+#pragma unroll
+        for (int k = 0; k < kShares; ++k) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1)
+                steps[k] += __shfl_xor_sync(0xffffffffu, steps[k], o);
+            if (lane == 0)
+                warp_steps[warp][k] = steps[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kShares; ++k) {
+            steps[k] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kPrepWarps; ++i)
+                steps[k] += warp_steps[i][k];
+        }
+        share = best_share(steps);
+    }
+    const float s = common_gain(top * p.temperature, share, p.inv_gain);
     if (blockIdx.x == 0 && warp == 0) {
         const BackShape shape = choose_shape(p.costs, p.t.rows, lane);
         if (lane == 0)
@@ -1203,7 +1350,14 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
     }
 
     const int vectors = p.width / 8;
-    for (int row = blockIdx.x * kPrepWarps + warp; row < p.t.rows; row += gridDim.x * kPrepWarps) {
+    for (int row = blockIdx.x * kPrepWarps + warp; row < p.g_rows; row += gridDim.x * kPrepWarps) {
+        if (row < lo_row + p.t.rows && row >= p.t.rows && row >= lo_row)
+            continue; // the second part: with the first
+        if (row >= p.t.rows) {
+            for (int i = lane; i < vectors; i += 32)
+                static_cast<uint4 *>(p.x_used)[static_cast<size_t>(row) * vectors + i] = make_uint4(0u, 0u, 0u, 0u);
+            continue;
+        }
         const size_t base = static_cast<size_t>(row) * vectors;
         const uint4 *src = static_cast<const uint4 *>(p.x) + base;
         uint4 *dst = static_cast<uint4 *>(p.x_used) + base;
@@ -1219,12 +1373,14 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
             p.row_lse2[row] = any ? p.lse[row] * kLog2e : 0.0f;
             p.row_gain[row] = any ? p.grad[row] * p.temperature * s : 0.0f;
         }
+        for (int part = 0; part <= (lo_row > 0); ++part, dst += static_cast<size_t>(lo_row) * vectors) {
 #pragma unroll
-        for (int i = 0; i < kHeadVectors; ++i)
-            if (lane + 32 * i < vectors)
-                dst[lane + 32 * i] = any ? head[i] : make_uint4(0u, 0u, 0u, 0u);
-        for (int i = lane + 32 * kHeadVectors; i < vectors; i += 32)
-            dst[i] = any ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < kHeadVectors; ++i)
+                if (lane + 32 * i < vectors)
+                    dst[lane + 32 * i] = any ? head[i] : make_uint4(0u, 0u, 0u, 0u);
+            for (int i = lane + 32 * kHeadVectors; i < vectors; i += 32)
+                dst[i] = any ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+        }
     }
 }
 
@@ -1249,17 +1405,7 @@ __device__ __forceinline__ float dot16(uint4 a, uint4 b, float acc)
     const uint32_t *u = &a.x, *v = &b.x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float2 p, q;
-        if (kBf16) {
-            p = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xFFFF0000u));
-            q = make_float2(__uint_as_float(v[i] << 16), __uint_as_float(v[i] & 0xFFFF0000u));
-        } else {
-            __half2 h, k;
-            memcpy(&h, &u[i], 4);
-            memcpy(&k, &v[i], 4);
-            p = __half22float2(h);
-            q = __half22float2(k);
-        }
+        const float2 p = unpack16(u[i], kBf16), q = unpack16(v[i], kBf16);
         acc = fmaf(p.x, q.x, acc);
         acc = fmaf(p.y, q.y, acc);
     }
@@ -1419,18 +1565,20 @@ __global__ void __launch_bounds__(32 * kCombineRowWarps) combine_rows_kernel(con
         write_row(p, row, mx, sum, target, label_z);
 }
 
-// dx = sum of the fp32 planes (one per K split), in order, times 1 / s; rows that moved come
-// from where they went, rows without a target are zero.  Eight elements per thread; blocks own
-// runs of kRows rows, and kRows rows of kPlanes planes are in flight together.
-template <bool kBf16, int kRows, int kPlanes>
+// dx = sum of the fp32 planes (one per K split; both parts' rows), in a fixed order, times 1 / s;
+// rows that moved come from where they went, rows without a target are zero.
+// Few planes, many rows: eight elements per thread, runs of four rows per block, in flight together.
+template <bool kBf16>
 __global__ void __launch_bounds__(256) planes_kernel(const float *planes, const BackShape *shape, int rows, int width,
                                                      const int *row_at, const float *inv_gain, uint4 *dx)
 {
+    constexpr int kRows = 4;
     // From the backward's first kernel, which the one before this waited for.
     const float inv = *inv_gain;
     const int vectors = width / 8;
-    const int count = shape->splits;
+    const int count = shape->splits, parts = shape->lo_row > 0 ? 2 : 1;
     const size_t plane = static_cast<size_t>(shape->plane_rows) * vectors; // in pairs of float4
+    const size_t part = static_cast<size_t>(shape->lo_row) * vectors;
     griddepcontrol_wait();
     griddepcontrol_launch_dependents();
     const float4 *all = reinterpret_cast<const float4 *>(planes);
@@ -1441,28 +1589,24 @@ __global__ void __launch_bounds__(256) planes_kernel(const float *planes, const 
             from[r] = row0 + r >= rows ? -1 : row_at ? row_at[row0 + r] : row0 + r;
         for (int i = threadIdx.x; i < vectors; i += blockDim.x) {
             float f[kRows][8] = {};
-            for (int s = 0; s < count; s += kPlanes) {
-                float4 v[kRows][kPlanes][2];
+            for (int s = 0; s < count * parts; ++s) {
+                float4 v[kRows][2];
 #pragma unroll
                 for (int r = 0; r < kRows; ++r)
-#pragma unroll
-                    for (int j = 0; j < kPlanes; ++j)
-                        if (from[r] >= 0 && s + j < count) {
-                            const float4 *src =
-                                all + 2 * (plane * (s + j) + static_cast<size_t>(from[r]) * vectors + i);
-                            v[r][j][0] = src[0];
-                            v[r][j][1] = src[1];
-                        } else {
-                            v[r][j][0] = v[r][j][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        }
-#pragma unroll
-                for (int r = 0; r < kRows; ++r)
-#pragma unroll
-                    for (int j = 0; j < kPlanes; ++j) {
-                        const float4 lo = v[r][j][0], hi = v[r][j][1];
-                        f[r][0] += lo.x, f[r][1] += lo.y, f[r][2] += lo.z, f[r][3] += lo.w;
-                        f[r][4] += hi.x, f[r][5] += hi.y, f[r][6] += hi.z, f[r][7] += hi.w;
+                    if (from[r] >= 0) {
+                        const float4 *src = all + 2 * (plane * (s / parts) + part * (s % parts) +
+                                                       static_cast<size_t>(from[r]) * vectors + i);
+                        v[r][0] = src[0];
+                        v[r][1] = src[1];
+                    } else {
+                        v[r][0] = v[r][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     }
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) {
+                    const float4 lo = v[r][0], hi = v[r][1];
+                    f[r][0] += lo.x, f[r][1] += lo.y, f[r][2] += lo.z, f[r][3] += lo.w;
+                    f[r][4] += hi.x, f[r][5] += hi.y, f[r][6] += hi.z, f[r][7] += hi.w;
+                }
             }
 #pragma unroll
             for (int r = 0; r < kRows; ++r)
@@ -1472,6 +1616,47 @@ __global__ void __launch_bounds__(256) planes_kernel(const float *planes, const 
                                    pack16(f[r][4] * inv, f[r][5] * inv, kBf16), pack16(f[r][6] * inv, f[r][7] * inv, kBf16));
         }
     }
+}
+
+// Many planes, few rows: a block sums one row's 256 columns, four per thread; its kPlaneGroups
+// groups of threads take every kPlaneGroups-th plane and meet in shared memory, so that a
+// thread waits for few loads in turn.
+constexpr int kPlaneColumns = 256, kPlaneGroups = 8;
+template <bool kBf16>
+__global__ void __launch_bounds__(kPlaneColumns / 4 * kPlaneGroups)
+    planes_row_kernel(const float *planes, const BackShape *shape, int width, const int *row_at, const float *inv_gain,
+                      uint2 *dx)
+{
+    __shared__ float4 sums[kPlaneGroups][kPlaneColumns / 4];
+    const float inv = *inv_gain;
+    const int row = blockIdx.y, group = threadIdx.y;
+    const int column = blockIdx.x * kPlaneColumns / 4 + threadIdx.x, columns = width / 4; // in float4
+    const int from = row_at ? row_at[row] : row;
+    const int lo_row = shape->lo_row, count = shape->splits;
+    const size_t plane = static_cast<size_t>(shape->plane_rows) * columns;
+    griddepcontrol_wait();
+    griddepcontrol_launch_dependents();
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](const float4 &v) { sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w; };
+    if (from >= 0 && column < columns) {
+        const float4 *src = reinterpret_cast<const float4 *>(planes) + static_cast<size_t>(from) * columns + column;
+        const size_t part = static_cast<size_t>(lo_row) * columns;
+#pragma unroll 5
+        for (int s = group; s < count; s += kPlaneGroups) {
+            add(src[plane * s]);
+            if (lo_row > 0)
+                add(src[plane * s + part]);
+        }
+    }
+    sums[group][threadIdx.x] = sum;
+    __syncthreads();
+    if (group != 0 || column >= columns)
+        return;
+#pragma unroll
+    for (int g = 1; g < kPlaneGroups; ++g)
+        add(sums[g][threadIdx.x]);
+    dx[static_cast<size_t>(row) * columns + column] =
+        make_uint2(pack16(sum.x * inv, sum.y * inv, kBf16), pack16(sum.z * inv, sum.w * inv, kBf16));
 }
 
 } // namespace vocab
@@ -1486,14 +1671,19 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Up to this many rows one CTA computes a tile instead of a pair: the rows fit one
-// accumulator and W is streamed once.  128 x 1280 x 51866: forward 29.6 us and backward 92 us,
-// with pairs 30.7 and 94.
+// accumulator and W is streamed once.  128 x 1280 x 51866: forward 28.7 us and backward 108 us,
+// with pairs 29.8 and 111.
 constexpr int64_t kSingleRows = 128;
 
 // Up to this many rows the forward's last step takes a warp per row; above, its strided reads
 // cost more than they save.  Whole forward over 384: 333 rows 22.2 us with a warp per row, 25.8
 // with 32 rows per block; 1024 rows 35.8 and 37.1; 2048 rows 71.5 and 66.0.
 constexpr int64_t kCombineRows = 1024;
+
+// Up to this many planes (or above kPlaneRows rows, a grid's y) dx is summed by runs of rows, else
+// a row at a time.  Backward by runs and by row: 2240 x 1024, one plane, 510 and 580 us; 1024 x
+// 384, five planes, 127 and 128; 700 x 384, six, 98 and 95; 333 x 384, nine, 74 and 65.
+constexpr int64_t kFewPlanes = 5, kPlaneRows = 65535;
 
 // Bytes of one piece of G: the memory a step may take for it, whatever its rows.  Larger pieces
 // are faster (14336 x 1280 x 51866: 6.07 ms with 256 MB, 5.94 with 512, 5.82 with all of G).
@@ -1593,10 +1783,18 @@ ForwardPlan plan_forward(const VocabLossLaunch &L, void *workspace)
 constexpr int64_t kTeacherMoveRows = 256;
 static_assert(kTeacherMoveRows == 32 * kPrepWarps, "prepare_teacher_kernel: a row per thread");
 
+// Rows that G and x_used have room for: all of a call's, or both parts of a few.
+int part_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+int64_t rows_of_g(int64_t rows)
+{
+    return std::max<int64_t>(rows, 2 * second_part(static_cast<int>(std::min<int64_t>(rows, kSplitRows)), part_rows(rows)));
+}
+
 struct BackwardPlan {
     bool single;             // kGrad by one CTA per tile
     bool moves;              // rows without a target are left out
     int targets;
+    int64_t g_rows;
     int64_t piece, pieces;   // vocabulary columns per piece of G
     int64_t ldg;             // elements per row of a piece
     int grad_bn, width_bn;   // tile widths over a piece's columns, and over x's width
@@ -1617,7 +1815,8 @@ BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
     b.single = L.rows <= kSingleRows;
     b.moves = L.targets == 0 || L.rows > kTeacherMoveRows;
     b.targets = L.targets > 0 ? L.targets : 1;
-    const int64_t most = std::max<int64_t>(256, kPieceBytes / 2 / L.rows / 256 * 256);
+    b.g_rows = rows_of_g(L.rows);
+    const int64_t most = std::max<int64_t>(256, kPieceBytes / 2 / b.g_rows / 256 * 256);
     b.pieces = ceil_div(L.vocab, most);
     b.piece = std::min(L.vocab, round_up(ceil_div(L.vocab, b.pieces), 256));
     b.pieces = ceil_div(L.vocab, b.piece);
@@ -1631,10 +1830,12 @@ BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
     b.costs.units = sm_count() / 2;
     b.costs.width = static_cast<int>(L.width);
     b.costs.plane_cap = INT_MAX;
+    b.costs.part_rows = part_rows(L.rows);
     float least = INFINITY;
     int kb_per = 1;
     for (int s = 1; s <= b.costs.units; ++s) {
-        const float cost = split_cost(b.costs, static_cast<int>(L.rows), s, kb_per);
+        const float cost =
+            split_cost(b.costs, static_cast<int>(L.rows <= kSplitRows ? b.g_rows : L.rows), s, kb_per);
         if (cost < least) {
             least = cost;
             b.splits = ceil_div(b.costs.kbs, kb_per);
@@ -1642,7 +1843,7 @@ BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
     }
     // Planes for those splits, or twice as many where that is at most 16 MB: fewer rows than
     // there can be may want more of them.
-    const int64_t plane_rows = b.splits * round_up(L.rows, 32);
+    const int64_t plane_rows = b.splits * round_up(b.g_rows, 32);
     b.costs.plane_cap = static_cast<int>(
         std::min<int64_t>(std::max(plane_rows, std::min(2 * plane_rows, (int64_t{16} << 20) / (4 * L.width))), INT_MAX));
     b.row_lse2 = arena.take<float>(L.rows);
@@ -1658,8 +1859,8 @@ BackwardPlan plan_backward(const VocabLossLaunch &L, void *workspace)
         b.sorted_prob = arena.take<float>(L.rows * b.targets);
     }
     b.shape = arena.take<BackShape>(1);
-    b.x_used = arena.take<uint16_t>(L.rows * L.width);
-    b.g = arena.take<uint16_t>(L.rows * b.ldg);
+    b.x_used = arena.take<uint16_t>(b.g_rows * L.width);
+    b.g = arena.take<uint16_t>(b.g_rows * b.ldg);
     if (L.dx)
         b.dx_planes = arena.take<float>(b.costs.plane_cap * L.width);
     b.bytes = arena.used;
@@ -1820,7 +2021,7 @@ cudaError_t launch_back(const VocabLossLaunch &L, const BackwardPlan &b, int64_t
 {
     CUtensorMap maps[6] = {};
     Params p{};
-    p.rows = static_cast<int>(L.rows);
+    p.rows = static_cast<int>(b.g_rows);
     p.shape = b.shape;
     p.n = static_cast<int>(L.width);
     p.bn = b.width_bn;
@@ -1834,18 +2035,18 @@ cudaError_t launch_back(const VocabLossLaunch &L, const BackwardPlan &b, int64_t
         const int64_t dims[2] = {L.width, b.costs.plane_cap};
         const int64_t strides[1] = {L.width * 4};
         const uint32_t box[2] = {16u, 32u};
-        if (!operand_map(&maps[0], kBf16, false, b.g, L.rows, cols, b.ldg, tile_rows(L.rows)) ||
+        if (!operand_map(&maps[0], kBf16, false, b.g, b.g_rows, cols, b.ldg, tile_rows(b.g_rows)) ||
             !operand_map(&maps[1], kBf16, true, w, cols, L.width, L.width, 0) ||
             !make_map_nd(&maps[2], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, b.dx_planes, dims, strides, box,
                          CU_TENSOR_MAP_SWIZZLE_64B))
             return cudaErrorInvalidValue;
         p.want_dx = 1;
-        tiles += 2 * b.splits * ceil_div(L.rows, 2 * kBM) * p.n_tiles;
+        tiles += 2 * b.splits * ceil_div(b.g_rows, 2 * kBM) * p.n_tiles;
     }
     if (L.dweight) {
         uint16_t *dw = static_cast<uint16_t *>(L.dweight) + col0 * L.width;
-        if (!operand_map(&maps[3], kBf16, true, b.g, L.rows, cols, b.ldg, 0) ||
-            !operand_map(&maps[4], kBf16, true, b.x_used, L.rows, L.width, L.width, 0) ||
+        if (!operand_map(&maps[3], kBf16, true, b.g, b.g_rows, cols, b.ldg, 0) ||
+            !operand_map(&maps[4], kBf16, true, b.x_used, b.g_rows, L.width, L.width, 0) ||
             !map16(&maps[5], kBf16, dw, cols, L.width, L.width, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B))
             return cudaErrorInvalidValue;
         p.dw_tiles = static_cast<int>(ceil_div(cols, 2 * kBM) * p.n_tiles);
@@ -1873,6 +2074,7 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
     q.ignore_index = L.ignore_index;
     q.temperature = L.temperature;
     q.width = static_cast<int>(L.width);
+    q.g_rows = static_cast<int>(b.g_rows);
     q.x = L.x;
     q.x_used = b.x_used;
     q.lse = L.lse_in;
@@ -1916,10 +2118,11 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
     for (int64_t col0 = 0; col0 < L.vocab; col0 += b.piece) {
         const int64_t cols = std::min(b.piece, L.vocab - col0);
         CUtensorMap out;
-        if (!map16(&out, kBf16, b.g, L.rows, cols, b.ldg, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B))
+        if (!map16(&out, kBf16, b.g, b.g_rows, cols, b.ldg, kSub, 32, CU_TENSOR_MAP_SWIZZLE_64B))
             return cudaErrorInvalidValue;
         Params p{};
         p.shape = b.shape;
+        p.g_rows = static_cast<int>(b.g_rows);
         p.t_index = b.t_index;
         p.t_prob = b.t_prob;
         p.targets = b.targets;
@@ -1932,16 +2135,23 @@ cudaError_t run_backward(const VocabLossLaunch &L, cudaStream_t stream)
             return err;
     }
     if (L.dx) {
-        // Few planes: four rows at a time (14336 x 1280, one plane: 20 us, with eight planes of one
-        // row 60); many, which means few rows: eight planes of one.
-        const bool few = b.splits <= 2;
-        const int64_t threads = std::min<int64_t>(round_up(L.width / 8, 32), 256);
-        const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, few ? 4 : 1), 4096 / threads * sm_count());
-        const auto kernel = few ? planes_kernel<kBf16, 4, 1> : planes_kernel<kBf16, 1, 8>;
-        err = launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(static_cast<unsigned>(threads)), stream,
-                         static_cast<const float *>(b.dx_planes), static_cast<const BackShape *>(b.shape),
-                         static_cast<int>(L.rows), static_cast<int>(L.width), static_cast<const int *>(b.row_at),
-                         static_cast<const float *>(b.inv_gain), static_cast<uint4 *>(L.dx));
+        const float *planes = b.dx_planes;
+        const BackShape *shape = b.shape;
+        const int *row_at = b.row_at;
+        const float *inv_gain = b.inv_gain;
+        const int width = static_cast<int>(L.width);
+        if (b.splits <= kFewPlanes || L.rows > kPlaneRows) {
+            const int64_t threads = std::min<int64_t>(round_up(L.width / 8, 32), 256);
+            const int64_t blocks = std::min<int64_t>(ceil_div(L.rows, 4), 4096 / threads * sm_count());
+            err = launch_pdl(planes_kernel<kBf16>, dim3(static_cast<unsigned>(blocks)),
+                             dim3(static_cast<unsigned>(threads)), stream, planes, shape, static_cast<int>(L.rows), width,
+                             row_at, inv_gain, static_cast<uint4 *>(L.dx));
+        } else {
+            err = launch_pdl(planes_row_kernel<kBf16>,
+                             dim3(static_cast<unsigned>(ceil_div(L.width, kPlaneColumns)), static_cast<unsigned>(L.rows)),
+                             dim3(kPlaneColumns / 4, kPlaneGroups), stream, planes, shape, width, row_at, inv_gain,
+                             static_cast<uint2 *>(L.dx));
+        }
     }
     return err;
 }

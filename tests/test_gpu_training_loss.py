@@ -155,7 +155,7 @@ def test_ignored_rows_reach_nothing(training, n, dtype):
 
 
 @pytest.mark.parametrize("teacher", [False, True])
-@pytest.mark.parametrize("n", [60, 500])
+@pytest.mark.parametrize("n", [60, 200, 500])
 def test_large_gradients_of_ignored_rows(training, n, teacher):
     """A finite but huge loss gradient at a row without a target scales nothing: neither fp16's
     range nor its precision is spent on it."""
@@ -230,6 +230,45 @@ def test_counts_of_valid_rows(training, n, valid):
     b_dx, b_dw = ref.grad_bounds(clean, w, grad, dloss, e_lse, e_dx, e_dw)
     assert not dx[out].any()
     assert ref.worst(dx, e_dx, b_dx) <= 1 and ref.worst(dw, e_dw, b_dw) <= 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,valid", [(1, 1), (7, 7), (8, 8), (8, 3), (9, 9), (16, 16), (17, 17), (33, 20), (100, 97),
+                                     (128, 128), (129, 128), (257, 1), (300, 9), (300, 33), (700, 64), (700, 128)])
+@pytest.mark.parametrize("teacher", [False, True])
+def test_few_rows_are_rounded_once(training, n, valid, teacher, dtype):
+    """With up to 128 rows that have a target (a teacher up to 256 rows: rows at all) the logits'
+    gradient is held in two parts, so that only the results are rounded to 16 bits."""
+    d, vocab, k = 72, 500, 3
+    g, x, w, dloss = operands(n, d, vocab, dtype, seed=valid)
+    out = torch.ones(n, dtype=torch.bool, device="cuda")
+    out[torch.randperm(n, generator=g, device="cuda")[:valid]] = False
+    x[out], dloss[out] = float("nan"), float("nan")
+    if teacher:
+        tokens = torch.randint(vocab, (n, k), generator=g, device="cuda", dtype=torch.int32)
+        tokens[out] = -1
+        logits = torch.randn((n, k), generator=g, device="cuda")
+        targets = ref.teacher_targets(tokens, logits, vocab, 1.0)
+        _, lse = training.distillation_forward(x, w, tokens, logits)
+        backward = lambda: training.distillation_backward(x, w, tokens, logits, lse, dloss)
+    else:
+        labels = torch.randint(vocab, (n,), generator=g, device="cuda")
+        labels[out] = -100
+        targets = ref.label_targets(labels, vocab, -100)
+        _, lse = training.cross_entropy_forward(x, w, labels)
+        backward = lambda: training.cross_entropy_backward(x, w, labels, lse, dloss)
+    poison = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(8)]
+    del poison  # the workspace's memory starts as NaN
+    dx, dw = backward()
+    clean = torch.where(out.unsqueeze(1), 0.0, x).to(dtype)
+    dloss = torch.where(out, 0.0, dloss)
+    _, e_lse, grad = ref.vocab_loss(clean, w, targets)
+    full = grad * dloss.double().unsqueeze(1)
+    e_dx, e_dw = full @ w.double(), full.t() @ clean.double()
+    parts = 1 if teacher and 128 < n <= 256 else 2
+    b_dx, b_dw = ref.grad_bounds(clean, w, grad, dloss, e_lse, e_dx, e_dw, 1.0, targets[0], k if teacher else 1, parts)
+    assert ref.worst(dx, e_dx, b_dx) <= 1 and ref.worst(dw, e_dw, b_dw) <= 1
+    assert not dx[out].any()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -127,11 +127,13 @@ def loss_bounds(x, weight, targets, losses, lse, temperature=1.0, entries=1):
     return temperature ** 2 * off + 2 * U32 * losses.abs(), off_lse
 
 
-def grad_bounds(x, weight, g, dloss, lse, dx, dweight, temperature=1.0, t=None, entries=1):
+def grad_bounds(x, weight, g, dloss, lse, dx, dweight, temperature=1.0, t=None, entries=1, parts=1):
     """G's error is p times the error of its exponent (the logit's, the given lse's rounding,
     the exponential's 2^-22), plus half a step of its 16-bit type, plus what the common scale
     2^13..2^14 over max |dloss T| flushes (2^-38 of that maximum); dx and dweight are sums of
     vocab or rows products of the tensor cores over it, rounded once.
+
+    With two parts G's rounding is that of what its rounding left off.
 
     With the targets t given, p is g / T + t itself, also where it exceeds a target.  A teacher's
     probabilities are off by 64 u at most, those of equal tokens together: exponents at a
@@ -152,7 +154,7 @@ def grad_bounds(x, weight, g, dloss, lse, dx, dweight, temperature=1.0, t=None, 
         soft = (g + temperature * t).clamp(min=0)
         target = temperature * (4 + 64 * (t > 0) * (entries > 1)) * U32
     big = (dloss.double().abs().max() * temperature) * 2.0 ** -38
-    off_g = gain * (soft * (torch.expm1(dz) + 2.0 ** -20) + target) + gain * g.abs() * (eps / 2) + big
+    off_g = gain * (soft * (torch.expm1(dz) + 2.0 ** -20) + target) + gain * g.abs() * (eps / 2) ** parts + big
     full = gain * g.abs()
     w, a = weight.double().abs(), x.double().abs()
     vocab, rows = weight.shape[0], x.shape[0]
