@@ -1078,7 +1078,7 @@ struct Prepare {
 
 // A rounding is off by up to half a step of its value's binade, which is least, relative to the
 // value, just under a power of two.  Most of G's weight is in the targets' elements, near -g T, so
-// of four gains a quarter of an octave apart the one is taken that rounds the g with the
+// of four gains a quarter of an octave apart the one is taken that rounds the g T with the
 // least squared error (loss gradients that are all alike then end up where steps are finest).
 constexpr int kShares = 4;
 __device__ __forceinline__ float gain_share(int i)
@@ -1086,7 +1086,7 @@ __device__ __forceinline__ float gain_share(int i)
     return i == 0 ? 1.0f : i == 1 ? 1.18920712f : i == 2 ? 1.41421356f : 1.68179283f;
 }
 
-// Adds the squared step of g times each share.
+// Adds the squared step of g (a loss gradient times T) times each share.
 __device__ __forceinline__ void add_steps(float (&steps)[kShares], float g)
 {
 #pragma unroll
@@ -1167,7 +1167,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
         top = fmaxf(top, g);
         before += used && i < begin;
         total += used;
-        add_steps(steps, g);
+        add_steps(steps, g * p.temperature);
     }
     reduce();
     if (lane == 0) {
@@ -1323,7 +1323,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
     float share = 1.0f;
     if (lo_row == 0) { // the rows known to have an entry decide
         float steps[kShares] = {};
-        add_steps(steps, known ? g : 0.0f);
+        add_steps(steps, known ? g * p.temperature : 0.0f);
 #pragma unroll
         for (int k = 0; k < kShares; ++k) {
 #pragma unroll
