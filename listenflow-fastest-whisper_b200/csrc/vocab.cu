@@ -2189,6 +2189,10 @@ cudaError_t read_and_clear_vocab_wait_error(int *site)
     int value = 0;
     cudaError_t err = cudaMemcpyFromSymbol(&value, g_device_error, sizeof(int));
     if (err == cudaSuccess && value != 0) {
+    // The copies follow the default stream's work only: what other streams hold is waited for first.
+    // A word that is set between the copies is part of the 1 that is then returned.
+    if (cudaDeviceSynchronize() != cudaSuccess)
+        return -1;
         const int zero = 0;
         err = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
     }
