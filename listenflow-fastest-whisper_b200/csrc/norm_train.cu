@@ -244,6 +244,7 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float *slot, int warps,
         v[0] = sum.x, v[N - 1] = sum.y;
     } else {
         v[0] = 0.0f;
+        __syncwarp(); // a barrier for memory too, as below: the caller may refill what was read
         for (int w = 0; w < warps; ++w)
             v[0] += slot[w];
     }
