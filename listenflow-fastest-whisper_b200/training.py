@@ -172,10 +172,10 @@ def _with_labels(a: native.VocabLossArgs, x: torch.Tensor, labels: torch.Tensor,
     a.temperature = 1.0
 
 
-def _with_teacher(a: native.VocabLossArgs, x: torch.Tensor, tokens: torch.Tensor, logits: torch.Tensor,
-                  temperature: float) -> None:
-    if (tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != a.rows
-            or not 1 <= tokens.shape[1] <= MAX_TEACHER_ENTRIES or tokens.device != x.device
+def _check_teacher(rows: int, device: torch.device, tokens: torch.Tensor, logits: torch.Tensor,
+                   temperature: float) -> None:
+    if (tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != rows
+            or not 1 <= tokens.shape[1] <= MAX_TEACHER_ENTRIES or tokens.device != device
             or not tokens.is_contiguous()):
         raise ValueError(f"teacher_tokens must be a contiguous int32 tensor [rows, 1 to {MAX_TEACHER_ENTRIES}] "
                          "on x's device")
@@ -196,6 +196,11 @@ def _workspace(a: native.VocabLossArgs, x: torch.Tensor, grad: int) -> torch.Ten
     a.workspace, a.workspace_bytes = workspace.data_ptr(), size
     return workspace
 
+
+
+def _with_teacher(a: native.VocabLossArgs, x: torch.Tensor, tokens: torch.Tensor, logits: torch.Tensor,
+                  temperature: float) -> None:
+    _check_teacher(a.rows, x.device, tokens, logits, temperature)
 
 def _loss_forward(a: native.VocabLossArgs, x: torch.Tensor, stream):
     device, rows = x.device, a.rows
