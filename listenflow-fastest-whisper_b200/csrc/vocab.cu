@@ -723,11 +723,7 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
                         if (next < step_end) {
                             const float z = select32(v, next - c0);
                             if (p.t_index) {
-                                // A weight of 0 (a repeated token's later entries, an exponential that
-                                // vanished) takes no part: z may be -infinity.
-                                const float weight = p.t_prob[static_cast<size_t>(row) * p.targets + entry];
-                                if (weight != 0.0f)
-                                    run_t = fmaf(weight, z, run_t);
+                                run_t = fmaf(p.t_prob[static_cast<size_t>(row) * p.targets + entry], z, run_t);
                                 ++entry;
                                 next = entry < p.targets ? row_cols[entry] - p.col0 : INT_MAX;
                             } else {
@@ -1115,19 +1111,16 @@ __device__ __forceinline__ float best_share(const float (&steps)[kShares])
     return share;
 }
 
-// The common gain s, a share times a power of two, puts max |g T s| in [2^13, 2^14) for any finite
-// g from 2^-100 on: with |p - t| <= 1, G then fits fp16 (65504) and keeps 11 bits down to
-// p = 2^-27 in the rows of the largest |g|, to 2^(k-27) in those of 2^-k of it.  Returns T s, since
-// g T alone may pass fp32's range; thread 0 of block 0 keeps 1 / s, by which the products' fp32
-// results are multiplied.  The exponent is taken of 2^-8 of the largest, which cannot overflow
-// (top < 2^128, T <= 2^6, share < 2).
-__device__ __forceinline__ float common_gain(float top, float temperature, float share, float *inv_gain)
+// The common gain s, a share times a power of two, puts max |g T s| in [2^13, 2^14): with
+// |p - t| <= 1, G then fits fp16 and keeps 11 bits down to p = 2^-28.  Returns s; thread 0 of
+// block 0 keeps 1 / s, by which the products' fp32 results are multiplied.
+__device__ __forceinline__ float common_gain(float top, float share, float *inv_gain)
 {
-    const int exponent = top > 0.0f ? min(max(ilogbf(top * 0x1p-8f * temperature * share) + 8, -100), 134) : 13;
+    const int exponent = top > 0.0f && top < INFINITY ? min(max(ilogbf(top * share), -100), 100) : 13;
     const float s = ldexpf(share, 13 - exponent);
     if (blockIdx.x == 0 && threadIdx.x == 0)
         *inv_gain = 1.0f / s;
-    return temperature * s;
+    return s;
 }
 
 constexpr int kHeadVectors = 5; // 1280 elements of a row per lane group, requested ahead
@@ -1193,7 +1186,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
     for (int k = 0; k < kShares; ++k)
         steps[k] = warp_steps[k][lane];
     reduce();
-    const float gain = common_gain(top, p.temperature, best_share(steps), p.inv_gain);
+    const float s = common_gain(top * p.temperature, best_share(steps), p.inv_gain);
     const int rows = max(total, 1), lo_row = second_part(rows, p.costs.part_rows); // a row of zeros where none has a target
     if (blockIdx.x == 0 && warp == 0) {
         const BackShape shape = choose_shape(p.costs, rows, lane);
@@ -1245,7 +1238,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
             }
             if (lane == 0) {
                 p.row_lse2[to] = p.lse[row] * kLog2e;
-                p.row_gain[to] = p.grad[row] * gain;
+                p.row_gain[to] = p.grad[row] * p.temperature * s;
             }
         }
         before += __popc(mask);
@@ -1349,7 +1342,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
         }
         share = best_share(steps);
     }
-    const float gain = common_gain(top, p.temperature, share, p.inv_gain);
+    const float s = common_gain(top * p.temperature, share, p.inv_gain);
     if (blockIdx.x == 0 && warp == 0) {
         const BackShape shape = choose_shape(p.costs, p.t.rows, lane);
         if (lane == 0)
@@ -1459,17 +1452,10 @@ __device__ __forceinline__ void write_row(const Combine &p, int row, float mx, f
         const int64_t label = load_label(p.labels, p.label_bytes, row);
         if (label >= 0 && label < p.vocab) {
             const double formed = p.label_z[row];
-            // One of the two sums may pass fp32's range on its way where the other does not: the
-            // finite one counts.
-            double z = label_z;
-            if (isfinite(formed) && isfinite(z))
-                lse -= exp(formed - lse) * (formed - z);
-            else if (isfinite(formed))
-                z = formed;
-            else if (isfinite(z)) // left out of the sum as -infinity
-                lse = fmax(lse, z) + log1p(exp(-fabs(lse - z)));
+            if (formed != label_z) // both may be infinite
+                lse -= exp(formed - lse) * (formed - label_z);
             if (label != p.ignore_index)
-                loss = lse - z;
+                loss = lse - label_z;
         } else if (label != p.ignore_index) {
             g_token_error = 1;
         }
@@ -2203,10 +2189,6 @@ cudaError_t read_and_clear_vocab_wait_error(int *site)
     int value = 0;
     cudaError_t err = cudaMemcpyFromSymbol(&value, g_device_error, sizeof(int));
     if (err == cudaSuccess && value != 0) {
-    // The copies follow the default stream's work only: what other streams hold is waited for first.
-    // A word that is set between the copies is part of the 1 that is then returned.
-    if (cudaDeviceSynchronize() != cudaSuccess)
-        return -1;
         const int zero = 0;
         err = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
     }
