@@ -350,7 +350,7 @@ LFFW_FP8_API lffw_status lffw_greedy_select(const uint16_t *logits, int64_t logi
                                             int32_t *tokens, int32_t *lengths, void *stream) LFFW_FP8_NOEXCEPT;
 
 /* Reads and clears the decoder kernels' error word: 0 none, 1 a token or position
- * outside its table, 2 a full cache.  Synchronises with the device. */
+ * outside its table, 2 a full cache.  Synchronises with the device, all its streams. */
 LFFW_FP8_API lffw_status lffw_decoder_error(int32_t *code) LFFW_FP8_NOEXCEPT;
 
 /* Q of an fp16 [rows, cols] weight with one scale per row (the per-output-channel
@@ -520,7 +520,7 @@ LFFW_FP8_API int64_t lffw_vocab_loss_workspace(const lffw_vocab_loss_args *args,
 LFFW_FP8_API lffw_status lffw_vocab_loss(const lffw_vocab_loss_args *args, void *stream) LFFW_FP8_NOEXCEPT;
 LFFW_FP8_API lffw_status lffw_vocab_loss_grad(const lffw_vocab_loss_args *args, void *stream) LFFW_FP8_NOEXCEPT;
 /* Reads and clears the current device's token error: 0 none, 1 a label or teacher token
- * outside the vocabulary.  Synchronises with the device. */
+ * outside the vocabulary.  Synchronises with the device, all its streams. */
 LFFW_FP8_API lffw_status lffw_vocab_loss_error(int32_t *code) LFFW_FP8_NOEXCEPT;
 
 /* GELU with every graph edge rounded to fp16, elementwise on `count` halves:

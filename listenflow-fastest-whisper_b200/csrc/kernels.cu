@@ -4304,6 +4304,9 @@ cudaError_t launch_greedy_select(const uint16_t *logits, int64_t logits_ld, cons
 
 int read_and_clear_decoder_error()
 {
+    // The copies follow the default stream's work only: what other streams hold is waited for first.
+    if (cudaDeviceSynchronize() != cudaSuccess)
+        return -1;
     int value = 0;
     if (cudaMemcpyFromSymbol(&value, dec::g_decoder_error, sizeof(int)) != cudaSuccess)
         return -1;

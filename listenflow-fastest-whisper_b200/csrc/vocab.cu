@@ -2175,6 +2175,10 @@ cudaError_t launch_vocab_loss_grad(const VocabLossLaunch &L, cudaStream_t stream
 
 int read_and_clear_token_error()
 {
+    // The copies follow the default stream's work only: what other streams hold is waited for first.
+    // A word that is set between the copies is part of the 1 that is then returned.
+    if (cudaDeviceSynchronize() != cudaSuccess)
+        return -1;
     int value = 0;
     if (cudaMemcpyFromSymbol(&value, vocab::g_token_error, sizeof(int)) != cudaSuccess)
         return -1;

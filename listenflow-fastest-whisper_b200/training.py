@@ -18,6 +18,7 @@ allocated on it.  Every byte of arithmetic runs in liblffw_b200.so.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -271,11 +272,14 @@ def distillation_backward(x: torch.Tensor, weight: torch.Tensor, teacher_tokens:
     return _loss_backward(a, x, weight, lse, dloss, want_dx, want_dweight, stream)
 
 
-def token_error() -> int:
-    """Reads and clears the device's token error: 1 when a label or teacher token outside the
-    vocabulary was met since the last call (it was treated as ignored), else 0."""
+def token_error(device: torch.device | int | str | None = None) -> int:
+    """Waits for the work queued on `device` (by default the current one), on any stream, then
+    reads and clears its token error: 1 when a label or teacher token outside the vocabulary was
+    met since the last call (it was treated as ignored), else 0.  A loss sets it on its tensors'
+    device."""
     code = ctypes.c_int32(0)
-    native.check(native.library().lffw_vocab_loss_error(ctypes.byref(code)), "lffw_vocab_loss_error")
+    with contextlib.nullcontext() if device is None else torch.cuda.device(device):
+        native.check(native.library().lffw_vocab_loss_error(ctypes.byref(code)), "lffw_vocab_loss_error")
     return int(code.value)
 
 
