@@ -723,7 +723,11 @@ __global__ void __launch_bounds__(Cfg<kPair, MODE>::kThreads, 1)
                         if (next < step_end) {
                             const float z = select32(v, next - c0);
                             if (p.t_index) {
-                                run_t = fmaf(p.t_prob[static_cast<size_t>(row) * p.targets + entry], z, run_t);
+                                // A weight of 0 (a repeated token's later entries, an exponential that
+                                // vanished) takes no part: z may be -infinity.
+                                const float weight = p.t_prob[static_cast<size_t>(row) * p.targets + entry];
+                                if (weight != 0.0f)
+                                    run_t = fmaf(weight, z, run_t);
                                 ++entry;
                                 next = entry < p.targets ? row_cols[entry] - p.col0 : INT_MAX;
                             } else {

@@ -1,0 +1,69 @@
+"""Edges of the scoring and training operators: weights of exactly zero, logits that pass fp32's
+range in one order of summation, loss gradients near the end of fp32's range, several pieces of
+the vocabulary, column sums over very many rows, and the whole tail against 64 bits."""
+
+from __future__ import annotations
+
+import importlib
+
+import pytest
+import torch
+
+import training_reference as ref
+from conftest import PACKAGE
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def training(cuda):
+    module = importlib.import_module(PACKAGE + ".training")
+    module.token_error()
+    yield module
+    assert module.token_error() == 0
+    assert importlib.import_module(PACKAGE + "._native").device_error() == 0
+
+
+def operands(n, d, vocab, dtype, seed=0, scale=0.1):
+    g = torch.Generator(device="cuda").manual_seed(seed + n * 7 + d * 3 + vocab)
+    x = torch.randn((n, d), generator=g, device="cuda").to(dtype)
+    w = (torch.randn((vocab, d), generator=g, device="cuda") * scale).to(dtype)
+    return g, x, w, torch.randn(n, generator=g, device="cuda")
+
+
+# ---- a teacher's weights of zero ------------------------------------------------------
+
+
+@pytest.mark.parametrize("n", [20, 300])
+@pytest.mark.parametrize("masked", [40, 300])
+def test_zero_weights_at_logits_of_minus_infinity(training, n, masked):
+    """A teacher's entry whose probability is exactly 0 says nothing about its token, whose logit
+    may be -infinity; a token there with a weight, once or repeated, costs an infinite loss."""
+    d, vocab = 64, 1200
+    g, x, w, dloss = operands(n, d, vocab, torch.bfloat16)
+    x[:, 0], w[:, 0] = 0.0, 0.0
+    tokens = torch.randint(masked, vocab, (n, 6), generator=g, device="cuda", dtype=torch.int32)
+    logits = torch.randn((n, 6), generator=g, device="cuda")
+    tokens[:, 2] = torch.randint(masked, (n,), generator=g, device="cuda", dtype=torch.int32)
+    logits[:, 2] = -1e4  # exp(-1e4) is 0 in fp32, and in 64 bits
+    left_out = tokens.clone()
+    left_out[:, 2] = -1
+    big = x.clone()
+    big[:, 0], w[:masked, 0] = 1e20, -1e20
+    losses, lse = training.distillation_forward(big, w, tokens, logits)
+    targets = ref.teacher_targets(left_out - masked, logits, vocab - masked, 1.0)
+    e_loss, e_lse, _ = ref.vocab_loss(x, w[masked:], targets)
+    b_loss, b_lse = ref.loss_bounds(x, w[masked:], targets, e_loss, e_lse, 1.0, 6)
+    assert ref.worst(lse, e_lse, b_lse) <= 1 and ref.worst(losses, e_loss, b_loss) <= 1
+    without, lse_without = training.distillation_forward(big, w, left_out, logits)
+    assert torch.equal(losses, without) and torch.equal(lse, lse_without)
+    grads = training.distillation_backward(big, w, tokens, logits, lse, dloss)
+    for a, b in zip(grads, training.distillation_backward(big, w, left_out, logits, lse, dloss)):
+        assert torch.equal(a, b)
+    # The same token twice and three times, among the masked ones, with weights above zero.
+    tokens[::2, 3:5] = tokens[::2, 2:3]
+    losses, lse = training.distillation_forward(big, w, tokens, logits)
+    assert losses[::2].isposinf().all() and ref.worst(lse, e_lse, b_lse) <= 1
+    assert torch.equal(losses[1::2], without[1::2])
