@@ -1456,10 +1456,17 @@ __device__ __forceinline__ void write_row(const Combine &p, int row, float mx, f
         const int64_t label = load_label(p.labels, p.label_bytes, row);
         if (label >= 0 && label < p.vocab) {
             const double formed = p.label_z[row];
-            if (formed != label_z) // both may be infinite
-                lse -= exp(formed - lse) * (formed - label_z);
+            // One of the two sums may pass fp32's range on its way where the other does not: the
+            // finite one counts.
+            double z = label_z;
+            if (isfinite(formed) && isfinite(z))
+                lse -= exp(formed - lse) * (formed - z);
+            else if (isfinite(formed))
+                z = formed;
+            else if (isfinite(z)) // left out of the sum as -infinity
+                lse = fmax(lse, z) + log1p(exp(-fabs(lse - z)));
             if (label != p.ignore_index)
-                loss = lse - label_z;
+                loss = lse - z;
         } else if (label != p.ignore_index) {
             g_token_error = 1;
         }

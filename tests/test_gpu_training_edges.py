@@ -67,3 +67,30 @@ def test_zero_weights_at_logits_of_minus_infinity(training, n, masked):
     losses, lse = training.distillation_forward(big, w, tokens, logits)
     assert losses[::2].isposinf().all() and ref.worst(lse, e_lse, b_lse) <= 1
     assert torch.equal(losses[1::2], without[1::2])
+
+
+# ---- sums that pass fp32's range on their way -------------------------------------------
+
+
+@pytest.mark.parametrize("n", [20, 200, 1500])
+def test_label_logits_whose_partial_sums_overflow(training, n):
+    """Products of 1.5 x 2^127 that cancel: two negative ones in the first sixteen columns, their
+    opposites 128 columns on.  A sum in the order of the columns passes -2^128 on its way, one of
+    pairs 128 apart does not; where it is the label's logit, its loss and lse are those of the
+    finite sum."""
+    d, vocab = 256, 900
+    g, x, w, _ = operands(n, d, vocab, torch.bfloat16)
+    hot = [0, 8, 128, 136]
+    x[:, hot], w[:, hot] = 0.0, 0.0
+    labels = torch.full((n,), 333, device="cuda")
+    labels[1::3] = torch.randint(vocab, (len(labels[1::3]),), generator=g, device="cuda")
+    labels[2::7] = -100
+    other = labels != 333
+    w[333, :16], w[333, 128:144] = 0.0, 0.0  # next to them, small products would be lost
+    targets = ref.label_targets(labels, vocab, -100)
+    e_loss, e_lse, _ = ref.vocab_loss(x, w, targets)
+    b_loss, b_lse = ref.loss_bounds(x, w, targets, e_loss, e_lse)
+    x[~other] = x[~other].index_fill(1, torch.tensor(hot, device="cuda"), 1.5 * 2.0 ** 63)
+    w[333, hot] = torch.tensor([-1.0, -1.0, 1.0, 1.0], device="cuda").bfloat16() * 2.0 ** 64
+    losses, lse = training.cross_entropy_forward(x, w, labels)
+    assert ref.worst(lse, e_lse, b_lse) <= 1 and ref.worst(losses, e_loss, b_loss) <= 1
