@@ -1115,16 +1115,19 @@ __device__ __forceinline__ float best_share(const float (&steps)[kShares])
     return share;
 }
 
-// The common gain s, a share times a power of two, puts max |g T s| in [2^13, 2^14): with
-// |p - t| <= 1, G then fits fp16 and keeps 11 bits down to p = 2^-28.  Returns s; thread 0 of
-// block 0 keeps 1 / s, by which the products' fp32 results are multiplied.
-__device__ __forceinline__ float common_gain(float top, float share, float *inv_gain)
+// The common gain s, a share times a power of two, puts max |g T s| in [2^13, 2^14) for any finite
+// g from 2^-100 on: with |p - t| <= 1, G then fits fp16 (65504) and keeps 11 bits down to
+// p = 2^-27 in the rows of the largest |g|, to 2^(k-27) in those of 2^-k of it.  Returns T s, since
+// g T alone may pass fp32's range; thread 0 of block 0 keeps 1 / s, by which the products' fp32
+// results are multiplied.  The exponent is taken of 2^-8 of the largest, which cannot overflow
+// (top < 2^128, T <= 2^6, share < 2).
+__device__ __forceinline__ float common_gain(float top, float temperature, float share, float *inv_gain)
 {
-    const int exponent = top > 0.0f && top < INFINITY ? min(max(ilogbf(top * share), -100), 100) : 13;
+    const int exponent = top > 0.0f ? min(max(ilogbf(top * 0x1p-8f * temperature * share) + 8, -100), 134) : 13;
     const float s = ldexpf(share, 13 - exponent);
     if (blockIdx.x == 0 && threadIdx.x == 0)
         *inv_gain = 1.0f / s;
-    return s;
+    return temperature * s;
 }
 
 constexpr int kHeadVectors = 5; // 1280 elements of a row per lane group, requested ahead
@@ -1190,7 +1193,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
     for (int k = 0; k < kShares; ++k)
         steps[k] = warp_steps[k][lane];
     reduce();
-    const float s = common_gain(top * p.temperature, best_share(steps), p.inv_gain);
+    const float gain = common_gain(top, p.temperature, best_share(steps), p.inv_gain);
     const int rows = max(total, 1), lo_row = second_part(rows, p.costs.part_rows); // a row of zeros where none has a target
     if (blockIdx.x == 0 && warp == 0) {
         const BackShape shape = choose_shape(p.costs, rows, lane);
@@ -1242,7 +1245,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) prepare_rows_kernel(const Prep
             }
             if (lane == 0) {
                 p.row_lse2[to] = p.lse[row] * kLog2e;
-                p.row_gain[to] = p.grad[row] * p.temperature * s;
+                p.row_gain[to] = p.grad[row] * gain;
             }
         }
         before += __popc(mask);
@@ -1346,7 +1349,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
         }
         share = best_share(steps);
     }
-    const float s = common_gain(top * p.temperature, share, p.inv_gain);
+    const float gain = common_gain(top, p.temperature, share, p.inv_gain);
     if (blockIdx.x == 0 && warp == 0) {
         const BackShape shape = choose_shape(p.costs, p.t.rows, lane);
         if (lane == 0)
@@ -1375,7 +1378,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) prepare_teacher_kernel(const 
         const bool any = sort_targets<R>(p.t, row, lane, probs[warp], keys[warp], entropy, total);
         if (lane == 0) {
             p.row_lse2[row] = any ? p.lse[row] * kLog2e : 0.0f;
-            p.row_gain[row] = any ? p.grad[row] * p.temperature * s : 0.0f;
+            p.row_gain[row] = any ? p.grad[row] * gain : 0.0f;
         }
         for (int part = 0; part <= (lo_row > 0); ++part, dst += static_cast<size_t>(lo_row) * vectors) {
 #pragma unroll

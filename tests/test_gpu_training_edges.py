@@ -94,3 +94,45 @@ def test_label_logits_whose_partial_sums_overflow(training, n):
     w[333, hot] = torch.tensor([-1.0, -1.0, 1.0, 1.0], device="cuda").bfloat16() * 2.0 ** 64
     losses, lse = training.cross_entropy_forward(x, w, labels)
     assert ref.worst(lse, e_lse, b_lse) <= 1 and ref.worst(losses, e_loss, b_loss) <= 1
+
+
+# ---- loss gradients near the end of fp32's range -----------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("teacher,temperature,exponent", [(False, 1.0, 90), (False, 1.0, 112), (False, 1.0, 127),
+                                                          (True, 1.0, 112), (True, 64.0, 110), (True, 64.0, 127),
+                                                          (True, 2.0 ** -6, 127)])
+@pytest.mark.parametrize("n", [20, 200, 300])
+def test_loss_gradients_near_the_end_of_the_range(training, n, teacher, temperature, exponent, dtype):
+    """Whatever the loss scale, the logits' gradient is held within its type: gradients that the
+    results' type holds are exact to their rounding, others are infinite with their sign, and a
+    column of zeros stays zero."""
+    d, vocab, k = 64, 300, 3
+    g, x, w, _ = operands(n, d, vocab, dtype)
+    x[:, 7], w[:, 5] = 0.0, 0.0
+    dloss = torch.where(torch.rand(n, generator=g, device="cuda") < 0.5, -1.0, 1.0) * 1.9 * 2.0 ** exponent
+    if teacher:
+        tokens = torch.randint(vocab, (n, k), generator=g, device="cuda", dtype=torch.int32)
+        logits = torch.randn((n, k), generator=g, device="cuda")
+        targets = ref.teacher_targets(tokens, logits, vocab, temperature)
+        _, lse = training.distillation_forward(x, w, tokens, logits, temperature=temperature)
+        dx, dw = training.distillation_backward(x, w, tokens, logits, lse, dloss, temperature=temperature)
+    else:
+        labels = torch.randint(vocab, (n,), generator=g, device="cuda")
+        targets = ref.label_targets(labels, vocab, -100)
+        _, lse = training.cross_entropy_forward(x, w, labels)
+        dx, dw = training.cross_entropy_backward(x, w, labels, lse, dloss)
+    assert not dx[:, 5].any() and not dw[:, 7].any()
+    _, e_lse, grad = ref.vocab_loss(x, w, targets, temperature)
+    full = grad * dloss.double().unsqueeze(1)
+    e_dx, e_dw = full @ w.double(), full.t() @ x.double()
+    bounds = ref.grad_bounds(x, w, grad, dloss, e_lse, e_dx, e_dw, temperature, targets[0], k if teacher else 1)
+    top = torch.finfo(dtype).max
+    for got, want, bound in zip((dx, dw), (e_dx, e_dw), bounds):
+        got = got.double()
+        inside = want.abs() + bound < top
+        assert ((got - want).abs() <= bound)[inside].all()
+        beyond = want.abs() - bound > top * (1 + torch.finfo(dtype).eps)
+        assert torch.equal(got[beyond], torch.copysign(torch.full_like(want[beyond], torch.inf), want[beyond]))
+        assert not torch.isnan(got).any()
