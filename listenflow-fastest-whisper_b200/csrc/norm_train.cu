@@ -224,6 +224,7 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float *slot, int warps,
 #pragma unroll
         for (int i = 0; i < N; ++i)
             v[i] = __shfl_sync(0xffffffffu, one, 32 / N * i);
+        __syncwarp(); // a barrier for memory too, as below: the caller may refill what was read
         return;
     }
     if (lane % (32 / N) == 0)

@@ -136,3 +136,30 @@ def test_loss_gradients_near_the_end_of_the_range(training, n, teacher, temperat
         beyond = want.abs() - bound > top * (1 + torch.finfo(dtype).eps)
         assert torch.equal(got[beyond], torch.copysign(torch.full_like(want[beyond], torch.inf), want[beyond]))
         assert not torch.isnan(got).any()
+
+
+# ---- norms whose rows one warp owns -------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [8, 64, 136, 256])
+def test_norms_of_one_warp_rows(training, cols, dtype):
+    """Rows that a single warp owns, in rings that are refilled many times (few stages of many
+    groups): the residual's gradient, which no sum uses, is read before its stage is."""
+    rows = 60001
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    normal = lambda *shape: torch.randn(shape, generator=g, device="cuda")
+    x, r, dy, dsum = (normal(rows, cols).to(dtype) for _ in range(4))
+    gamma, beta = 1 + 0.2 * normal(cols), 0.3 * normal(cols)
+    total, y, stats = training.layer_norm_forward(x, gamma, beta, residual=r)
+    dx, dgamma, dbeta = training.layer_norm_backward(dy, total, gamma, stats, dsum=dsum)
+    e_total, e_y, mean, rstd = ref.layer_norm(x, gamma, beta, 1e-5, r)
+    assert torch.equal(total, e_total)
+    assert ref.worst(y, e_y, ref.layer_norm_bound(total, gamma, beta, e_y, mean, rstd)) <= 1
+    e = ref.layer_norm_grads(dy, total, gamma, mean, rstd, dsum)
+    b = ref.layer_norm_grad_bounds(dy, total, gamma, mean, rstd, e[0], dsum)
+    for got, want, bound in zip((dx, dgamma, dbeta), e, b):
+        assert ref.worst(got, want, bound) <= 1
+    for _ in range(20):
+        again = training.layer_norm_backward(dy, total, gamma, stats, dsum=dsum)
+        assert all(torch.equal(a, b) for a, b in zip(again, (dx, dgamma, dbeta)))
