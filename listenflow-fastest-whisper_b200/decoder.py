@@ -396,14 +396,16 @@ class Decoder:
                    temperature: float = 1.0, start_token: int = SOT,
                    ignore_index: int = training.IGNORE_INDEX) -> torch.Tensor:
         """T^2 KL(teacher || this decoder) per token of given transcripts, fp32 [streams,
-        length], 0 for padding, from a teacher's best logits [streams, length, k] (int32 tokens,
-        fp16/bf16/fp32 logits): how far quantisation has moved a decoder from the one it was
+        length], 0 for padding, from a teacher's best logits [streams, length, k] (int32 or int64
+        tokens, fp16/bf16/fp32 logits): how far quantisation has moved a decoder from the one it was
         made of, token by token."""
         if (teacher_tokens.dim() != 3 or teacher_tokens.shape[:2] != transcripts.shape
                 or teacher_logits.shape != teacher_tokens.shape):
             raise ValueError("teacher_tokens and teacher_logits must be [streams, length, k] like transcripts")
         states = self.final_states(transcripts, start_token, ignore_index)
         k = teacher_tokens.shape[2]
+        if teacher_tokens.dtype == torch.int64:  # topk's indices: none may come back inside the vocabulary
+            teacher_tokens = teacher_tokens.clamp(-1, torch.iinfo(torch.int32).max)
         tokens = torch.where((transcripts == ignore_index).unsqueeze(2), -1, teacher_tokens).to(torch.int32)
         losses, _ = training.distillation_forward(
             states.view(-1, self.config.d_model), self.weights.token_table,
