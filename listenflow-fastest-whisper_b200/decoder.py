@@ -354,14 +354,17 @@ class Decoder:
         0 .. t - 1.  Leaves the caches holding the transcripts' tokens but the last.  A token
         outside the vocabulary sets fp8.decoder_error: what follows it in its transcript counts
         for nothing."""
+        self._check_transcripts(transcripts)
+        with torch.cuda.device(self.tokens.device):
+            return self._final_states(transcripts, start_token, ignore_index)
+
+    def _check_transcripts(self, transcripts: torch.Tensor) -> None:
         c, s = self.config, self.streams
         if (transcripts.dtype != torch.int32 or transcripts.dim() != 2 or transcripts.shape[0] != s
                 or transcripts.device != self.tokens.device
                 or not 1 <= transcripts.shape[1] <= min(self.capacity, c.positions)):
             raise ValueError(f"transcripts must be int32 [{s}, 1 to {min(self.capacity, c.positions)}] on "
                              f"{self.tokens.device}")
-        with torch.cuda.device(self.tokens.device):
-            return self._final_states(transcripts, start_token, ignore_index)
 
     def _final_states(self, transcripts: torch.Tensor, start_token: int, ignore_index: int) -> torch.Tensor:
         c, s = self.config, self.streams
@@ -402,15 +405,20 @@ class Decoder:
         if (teacher_tokens.dim() != 3 or teacher_tokens.shape[:2] != transcripts.shape
                 or teacher_logits.shape != teacher_tokens.shape):
             raise ValueError("teacher_tokens and teacher_logits must be [streams, length, k] like transcripts")
-        states = self.final_states(transcripts, start_token, ignore_index)
+        self._check_transcripts(transcripts)
+        if teacher_tokens.device != transcripts.device:
+            raise ValueError(f"teacher_tokens must be on {transcripts.device}")
         k = teacher_tokens.shape[2]
         if teacher_tokens.dtype == torch.int64:  # topk's indices: none may come back inside the vocabulary
             teacher_tokens = teacher_tokens.clamp(-1, torch.iinfo(torch.int32).max)
         tokens = torch.where((transcripts == ignore_index).unsqueeze(2), -1, teacher_tokens).to(torch.int32)
-        losses, _ = training.distillation_forward(
-            states.view(-1, self.config.d_model), self.weights.token_table,
-            tokens.transpose(0, 1).reshape(-1, k).contiguous(),
-            teacher_logits.transpose(0, 1).reshape(-1, k).contiguous(), temperature=temperature)
+        rows = transcripts.numel()
+        tokens = tokens.transpose(0, 1).reshape(rows, k).contiguous()
+        logits = teacher_logits.transpose(0, 1).reshape(rows, k).contiguous()
+        training._check_teacher(rows, tokens.device, tokens, logits, temperature)  # before the decode
+        states = self.final_states(transcripts, start_token, ignore_index)
+        losses, _ = training.distillation_forward(states.view(-1, self.config.d_model), self.weights.token_table,
+                                                  tokens, logits, temperature=temperature)
         return losses.view(transcripts.shape[1], self.streams).t()
 
 

@@ -173,18 +173,23 @@ def _with_labels(a: native.VocabLossArgs, x: torch.Tensor, labels: torch.Tensor,
     a.temperature = 1.0
 
 
-def _with_teacher(a: native.VocabLossArgs, x: torch.Tensor, tokens: torch.Tensor, logits: torch.Tensor,
-                  temperature: float) -> None:
-    if (tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != a.rows
-            or not 1 <= tokens.shape[1] <= MAX_TEACHER_ENTRIES or tokens.device != x.device
+def _check_teacher(rows: int, device: torch.device, tokens: torch.Tensor, logits: torch.Tensor,
+                   temperature: float) -> None:
+    if (tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != rows
+            or not 1 <= tokens.shape[1] <= MAX_TEACHER_ENTRIES or tokens.device != device
             or not tokens.is_contiguous()):
         raise ValueError(f"teacher_tokens must be a contiguous int32 tensor [rows, 1 to {MAX_TEACHER_ENTRIES}] "
                          "on x's device")
-    if (logits.dtype not in _TEACHER_DTYPES or logits.shape != tokens.shape or logits.device != x.device
+    if (logits.dtype not in _TEACHER_DTYPES or logits.shape != tokens.shape or logits.device != device
             or not logits.is_contiguous()):
         raise ValueError("teacher_logits must be a contiguous float16, bfloat16 or float32 tensor like teacher_tokens")
     if not 2.0 ** -6 <= temperature <= 2.0 ** 6:
         raise ValueError("temperature must lie in [2^-6, 2^6]")
+
+
+def _with_teacher(a: native.VocabLossArgs, x: torch.Tensor, tokens: torch.Tensor, logits: torch.Tensor,
+                  temperature: float) -> None:
+    _check_teacher(a.rows, x.device, tokens, logits, temperature)
     a.teacher_entries, a.teacher_dtype = tokens.shape[1], _TEACHER_DTYPES[logits.dtype]
     a.teacher_tokens, a.teacher_logits, a.temperature = tokens.data_ptr(), logits.data_ptr(), temperature
 

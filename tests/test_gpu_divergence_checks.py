@@ -1,4 +1,4 @@
-"""Decoder.divergence: a teacher's tokens of 64 bits."""
+"""Decoder.divergence: a teacher's tokens of 64 bits, and refusals that come before the decode."""
 
 from __future__ import annotations
 
@@ -45,3 +45,22 @@ def test_tokens_of_64_bits(plan, transcripts):
         tokens[0, 1, 2] = bad
         assert torch.equal(plan.divergence(transcripts, tokens, logits), plan.divergence(transcripts, left_out, logits))
         assert training.token_error() == (1 if bad > 0 else 0)
+
+
+def test_refusals_leave_the_plan(plan, transcripts):
+    """A call that is refused has decoded nothing: the caches stay as they were."""
+    tokens = torch.zeros((STREAMS, LENGTH, 4), dtype=torch.int32, device="cuda")
+    logits = torch.zeros((STREAMS, LENGTH, 4), device="cuda")
+    plan.reset()
+    for call in (lambda: plan.divergence(transcripts, tokens, logits.double()),
+                 lambda: plan.divergence(transcripts, tokens, logits.cpu()),
+                 lambda: plan.divergence(transcripts, tokens.cpu(), logits),
+                 lambda: plan.divergence(transcripts.long(), tokens, logits),
+                 lambda: plan.divergence(transcripts.cpu(), tokens, logits),
+                 lambda: plan.divergence(transcripts, tokens[..., :0], logits[..., :0]),
+                 lambda: plan.divergence(transcripts, tokens.repeat(1, 1, 65), logits.repeat(1, 1, 65)),
+                 lambda: plan.divergence(transcripts, tokens, logits, temperature=0.0),
+                 lambda: plan.divergence(transcripts, tokens, logits, temperature=float("nan"))):
+        with pytest.raises(ValueError):
+            call()
+        assert not plan.lengths.any()
