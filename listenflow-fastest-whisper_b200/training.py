@@ -13,7 +13,11 @@ over the vocabulary.
 Rows are fp16 or bf16, LayerNorm parameters, losses and log-sum-exps fp32.  Tensors are
 contiguous CUDA tensors of one device; the work is queued on ``stream`` (a torch stream or a
 cudaStream_t), by default that device's current stream, and results and workspaces are
-allocated on it.  Every byte of arithmetic runs in liblffw_b200.so.
+allocated on it.  Inputs made on other streams are the caller's to wait for; they may be let
+go of once a call returns if ``stream`` is a torch stream (their memory is recorded on it),
+and with a cudaStream_t, or without ``stream`` where the current stream is not theirs, once
+the work has run, as for any torch operator.  Every byte of arithmetic runs in
+liblffw_b200.so.
 """
 
 from __future__ import annotations
@@ -43,8 +47,10 @@ def _elsewhere(device: torch.device, stream) -> bool:
     return stream is not None or device.index != _current_device()
 
 
-def _scope(device: torch.device, stream):
-    """Makes `device` and `stream` current: allocations follow the current stream."""
+def _scope(device: torch.device, stream, *inputs: torch.Tensor | None):
+    """Makes `device` and `stream` current: allocations follow the current stream.  The memory of
+    `inputs` is kept from other uses until a torch stream has read it, should the caller let go
+    of them; a cudaStream_t's life is its owner's, so nothing is recorded on one."""
     if stream is None:
         return torch.cuda.device(device)
     if not isinstance(stream, torch.cuda.Stream):
@@ -52,6 +58,11 @@ def _scope(device: torch.device, stream):
         stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
     if stream.device != device:
         raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
+    # A stream object around a handle has the handle as its id (the default stream's are 0 both).
+    if stream.stream_id != stream.cuda_stream or stream.cuda_stream == 0:
+        for t in inputs:
+            if t is not None:
+                t.record_stream(stream)
     return torch.cuda.stream(stream)
 
 
@@ -99,7 +110,7 @@ def layer_norm_forward(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor,
     if residual is not None:
         _like(residual, x, "residual", "x")
     if _elsewhere(device, stream):
-        with _scope(device, stream):
+        with _scope(device, stream, x, gamma, beta, residual):
             return layer_norm_forward(x, gamma, beta, eps, residual=residual)
     total = x if residual is None else torch.empty_like(x)
     y = torch.empty_like(x)
@@ -132,7 +143,7 @@ def layer_norm_backward(dy: torch.Tensor, total: torch.Tensor, gamma: torch.Tens
     if not want_dx and not want_params:
         raise ValueError("nothing to compute: want_dx and want_params are both false")
     if _elsewhere(device, stream):
-        with _scope(device, stream):
+        with _scope(device, stream, dy, total, gamma, stats, dsum):
             return layer_norm_backward(dy, total, gamma, stats, dsum=dsum, want_dx=want_dx, want_params=want_params)
     dx = torch.empty_like(total) if want_dx else None
     dgamma = dbeta = workspace = None
@@ -203,10 +214,10 @@ def _workspace(a: native.VocabLossArgs, x: torch.Tensor, grad: int) -> torch.Ten
     return workspace
 
 
-def _loss_forward(a: native.VocabLossArgs, x: torch.Tensor, stream):
+def _loss_forward(a: native.VocabLossArgs, x: torch.Tensor, stream, *others: torch.Tensor):
     device, rows = x.device, a.rows
     if _elsewhere(device, stream):
-        with _scope(device, stream):
+        with _scope(device, stream, x, *others):
             return _loss_forward(a, x, None)
     losses = torch.empty(rows, dtype=torch.float32, device=device)
     lse = torch.empty_like(losses)
@@ -218,14 +229,14 @@ def _loss_forward(a: native.VocabLossArgs, x: torch.Tensor, stream):
 
 
 def _loss_backward(a: native.VocabLossArgs, x: torch.Tensor, weight: torch.Tensor, lse: torch.Tensor,
-                   dloss: torch.Tensor, want_dx: bool, want_dweight: bool, stream):
+                   dloss: torch.Tensor, want_dx: bool, want_dweight: bool, stream, *targets: torch.Tensor):
     device, rows = x.device, a.rows
     _vector(lse, _FLOAT, rows, device, "lse")
     _vector(dloss, _FLOAT, rows, device, "dloss")
     if not want_dx and not want_dweight:
         raise ValueError("nothing to compute: want_dx and want_dweight are both false")
     if _elsewhere(device, stream):
-        with _scope(device, stream):
+        with _scope(device, stream, x, weight, lse, dloss, *targets):
             return _loss_backward(a, x, weight, lse, dloss, want_dx, want_dweight, None)
     dx = torch.empty_like(x) if want_dx else None
     if not rows:
@@ -245,7 +256,7 @@ def cross_entropy_forward(x: torch.Tensor, weight: torch.Tensor, labels: torch.T
     labels: int32 or int64 [rows]; a row labelled `ignore_index` has loss 0."""
     a = _operands(x, weight)
     _with_labels(a, x, labels, ignore_index)
-    return _loss_forward(a, x, stream)
+    return _loss_forward(a, x, stream, weight, labels)
 
 
 def cross_entropy_backward(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor,
@@ -254,7 +265,7 @@ def cross_entropy_backward(x: torch.Tensor, weight: torch.Tensor, labels: torch.
     """(dx, dweight) in x's type from the forward's lse and the losses' gradients dloss."""
     a = _operands(x, weight)
     _with_labels(a, x, labels, ignore_index)
-    return _loss_backward(a, x, weight, lse, dloss, want_dx, want_dweight, stream)
+    return _loss_backward(a, x, weight, lse, dloss, want_dx, want_dweight, stream, labels)
 
 
 def distillation_forward(x: torch.Tensor, weight: torch.Tensor, teacher_tokens: torch.Tensor,
@@ -265,7 +276,7 @@ def distillation_forward(x: torch.Tensor, weight: torch.Tensor, teacher_tokens: 
     entry left out), teacher_logits fp16, bf16 or fp32 [rows, k]."""
     a = _operands(x, weight)
     _with_teacher(a, x, teacher_tokens, teacher_logits, temperature)
-    return _loss_forward(a, x, stream)
+    return _loss_forward(a, x, stream, weight, teacher_tokens, teacher_logits)
 
 
 def distillation_backward(x: torch.Tensor, weight: torch.Tensor, teacher_tokens: torch.Tensor,
@@ -274,7 +285,7 @@ def distillation_backward(x: torch.Tensor, weight: torch.Tensor, teacher_tokens:
     """(dx, dweight) in x's type from the forward's lse and the losses' gradients dloss."""
     a = _operands(x, weight)
     _with_teacher(a, x, teacher_tokens, teacher_logits, temperature)
-    return _loss_backward(a, x, weight, lse, dloss, want_dx, want_dweight, stream)
+    return _loss_backward(a, x, weight, lse, dloss, want_dx, want_dweight, stream, teacher_tokens, teacher_logits)
 
 
 def token_error(device: torch.device | int | str | None = None) -> int:
