@@ -64,11 +64,16 @@ def test_inputs_that_are_let_go_of(training, inputs, name):
     block = torch.empty((8192, 8192), device="cuda", dtype=torch.bfloat16).normal_()
     out = torch.empty_like(block)
     side = torch.cuda.Stream()
+    # The call's memory is there beforehand: an allocation that has to give cached memory back waits
+    # for every stream.
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    call(side, fixed)
     args = {k: v.clone() for k, v in fixed.items()}
     taken = {k: (v.data_ptr(), v.numel() * v.element_size()) for k, v in args.items()}
     torch.cuda.synchronize()
-    with torch.cuda.stream(side):  # some 30 ms of work before the call
-        for _ in range(40):
+    with torch.cuda.stream(side):  # some 70 ms of work before the call
+        for _ in range(100):
             torch.mm(block, block, out=out)
     got = [t for t in call(side, args) if t is not None]
     shapes = [v.shape for v in args.values()], [v.dtype for v in args.values()]
