@@ -407,7 +407,8 @@ LFFW_FP8_API lffw_status lffw_pack_skinny_weights(const void *weight, int64_t n,
  * transcripts and to tune its norms and token table.  Rows are fp16 or bf16 (`dtype`,
  * LFFW_DT_HALF or LFFW_DT_BF16); arithmetic is fp32.  Results do not depend on timing:
  * no floating-point sum is formed in an order that varies between runs.  Every call
- * waits for the work before it on `stream` before it reads anything, weights included.
+ * waits for the work before it on `stream` before it reads anything, weights included (its
+ * later kernels read inputs early, once its first kernel has waited).
  * Calls on the same stream may share a workspace; calls that may overlap may not.
  * Inputs, outputs and workspace may not overlap one another unless said otherwise.
  *
@@ -484,9 +485,12 @@ LFFW_FP8_API lffw_status lffw_layer_norm_grad(const lffw_layer_norm_grad_args *a
  * lffw_vocab_loss_grad reads lse and dloss (fp32 [rows], the gradients of the losses)
  * and writes, in `dtype`, dx [rows, width] and/or dweight [vocab, width]:
  *   G = dloss T (exp(z / T - lse) - t),  dx = G weight,  dweight = G^T x
- * G is formed piece by piece over the vocabulary and held in 16 bits, scaled so that fp16
- * neither overflows nor loses small probabilities; where at most 128 rows have a target, in
- * twice 16 bits.  Sums are fp32.
+ * G is formed piece by piece over the vocabulary (512 MB at most for up to 2^20 rows; at
+ * least 256 columns) and held in 16 bits, scaled in common so that fp16 does not overflow for
+ * any finite dloss and holds its 11 bits down to probabilities of 2^-27 in the rows of the
+ * largest |dloss|, 2^(k-27) in rows of 2^-k of that.  Where at most 128 rows have a target, G
+ * is held in twice 16 bits (with a teacher and 129 to 256 rows, all rows count as having
+ * one).  Sums are fp32.
  * workspace holds lffw_vocab_loss_workspace(args, 0 for the loss, 1 for the gradients)
  * bytes (-1 for invalid arguments; it depends on the current device, the shape, the number
  * of targets and, for the gradients, on which of dx and dweight are set, never on contents).

@@ -165,8 +165,8 @@ struct Ring {
     // One thread, once all of the group have read the current stage: requests the rows from row0 on
     // into it.  Where the wait gave up, the copies in flight are waited for first, in a group's last
     // steps too, so that none lands after the block has left its shared memory or reuses it.  (The
-    // test's time is within the noise: 96000 x 1280, 176 and 156 us without it, 170 and 152 with it;
-    // the same after the steps instead of in them kept registers from these: 182 and 189.)
+    // test costs nothing: 96000 x 1280, each direction alone, 176 and 156 us without it, 170 and 152
+    // with it; the same after the steps instead of in them kept registers from these: 182 and 189.)
     __device__ __forceinline__ void refill(int64_t row0) const
     {
         if (mbar_test(bars + 8 * stage, phase) || landed_late(bars + 8 * stage, phase))

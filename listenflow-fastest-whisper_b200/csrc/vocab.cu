@@ -14,7 +14,7 @@
 //            vocabulary columns)
 //   kBack    that piece times its rows of W (dx, summed over the pieces in fp32) and that piece
 //            transposed times x (its rows of dW), one list of tiles shared out over the SMs
-// A piece of G is the only n x (part of V) tensor that ever exists.
+// A piece of G is the only n x (part of V) tensor that ever exists (all of V where 512 MB hold it).
 //
 // Rows without a target are left out of the gradients' products altogether.
 //
@@ -1797,7 +1797,10 @@ ForwardPlan plan_forward(const VocabLossLaunch &L, void *workspace)
 constexpr int64_t kTeacherMoveRows = 256;
 static_assert(kTeacherMoveRows == 32 * kPrepWarps, "prepare_teacher_kernel: a row per thread");
 
-// Rows that G and x_used have room for: all of a call's, or both parts of a few.
+// Rows that G and x_used have room for: all of a call's, or both parts of a few.  A part of 8 or 16
+// rows, where a call has no more, puts both into one store of 32.  Backward over 51865 tokens with
+// those and with 32 always, us: 1 x 384 39.9 and 41.0; 7 x 512 of 5 teacher's entries 46.2 and 47.7;
+// 16 x 1280 96.1 and 96.8.
 int part_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 int64_t rows_of_g(int64_t rows)
 {

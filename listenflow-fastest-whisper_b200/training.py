@@ -6,9 +6,10 @@
 
 Each has a ``*_forward`` and a ``*_backward`` call, which allocate nothing but their results
 and a workspace, and an autograd form of its plain name.  The two losses take the final
-states [n, width] and the token table [vocab, width] (tied embedding and logits weight);
-neither the logits nor their gradient is ever held: the gradients are formed piece by piece
-over the vocabulary.
+states [n, width] and the token table [vocab, width] (tied embedding and logits weight).
+The logits are never held; their gradient is, in 16 bits, a piece of the vocabulary at a time
+(512 MB at most for up to 2^20 rows, which up to some 5000 rows of a 51866-token table is
+all of it).
 
 Rows are fp16 or bf16, LayerNorm parameters, losses and log-sum-exps fp32.  Tensors are
 contiguous CUDA tensors of one device; the work is queued on ``stream`` (a torch stream or a

@@ -1,7 +1,7 @@
 /*
  * CPU oracle for the FP8 E4M3 quantized-linear path and the fp16 projection
  * plugins.  TEST INFRASTRUCTURE ONLY: tests/, __graft_entry__.smoke() and the
- * cpu_baseline / reference arm of bench.py use it as the checker.  The product
+ * cpu_baseline / reference arm of bench.py use it as the oracle.  The product
  * library (liblffw_b200.so) never links or calls it.
  *
  * Every routine restates the reference's arithmetic in plain C:
