@@ -311,6 +311,26 @@ def _grad(g: torch.Tensor | None) -> torch.Tensor | None:
     return g if g.data_ptr() % 16 == 0 else g.clone()
 
 
+# Casts and views between an input and its leaf that _guard_capture looks through.
+_GUARDED_STEPS = 8
+
+
+def _accumulator(t: torch.Tensor):
+    """The gradient accumulator of a leaf, also where t is made from it alone by a few casts or
+    views (a 16-bit copy of 32-bit weights); None for other tensors."""
+    if t.is_leaf:
+        return torch.autograd.graph.get_gradient_edge(t).node
+    node = t.grad_fn
+    for _ in range(_GUARDED_STEPS):
+        before = [n for n, _ in node.next_functions if n is not None]
+        if len(before) != 1:
+            return None
+        node = before[0]
+        if node.name() == "torch::autograd::AccumulateGrad":
+            return node
+    return None
+
+
 def _guard_capture(*inputs: torch.Tensor | None) -> list:
     """Refuses to record, in a CUDA graph capture, an autograd graph over a leaf that an eager
     graph of these operators still holds: the engine would join the eager graph's stream to
@@ -318,14 +338,20 @@ def _guard_capture(*inputs: torch.Tensor | None) -> list:
     lives as long as a graph holds it, and so does the mark left on it here.  Returns the
     accumulators, for the caller to hold until the new graph does."""
     accumulators = []
-    leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf and t.is_cuda]
-    if not leaves or not torch.is_grad_enabled():
+    if not torch.is_grad_enabled():
         return accumulators
-    capturing = torch.cuda.is_current_stream_capturing()
-    for leaf in leaves:
-        accumulators.append(torch.autograd.graph.get_gradient_edge(leaf).node)
-        mark = accumulators[-1].metadata
-        stream = torch.cuda.current_stream(leaf.device).cuda_stream
+    capturing = None
+    for t in inputs:
+        if t is None or not t.requires_grad or not t.is_cuda:
+            continue
+        accumulator = _accumulator(t)
+        if accumulator is None:
+            continue
+        accumulators.append(accumulator)
+        if capturing is None:
+            capturing = torch.cuda.is_current_stream_capturing()
+        mark = accumulator.metadata
+        stream = torch.cuda.current_stream(t.device).cuda_stream
         if capturing and mark.get("lffw_stream", stream) != stream:
             raise RuntimeError(
                 "an eager autograd graph of this leaf is alive: release its losses before capturing a backward "
